@@ -12,7 +12,7 @@ step runs hand-written HIP kernels for gfx950 (libgoi_b2.so through the C ABI in
 """
 import numpy as np
 
-from . import debug, io, layout, record, scenes, shapes, world
+from . import debug, io, layout, policy, record, scenes, shapes, world
 from .settings import Settings
 from .step import (collide_, debug_shapes, last_launch, make_debug, prepare, sincos, step, step_, step_n_,
                    world_manifolds)
@@ -25,4 +25,4 @@ __all__ = ["Settings", "step", "step_", "step_n_", "collide_", "debug_shapes", "
            "sincos", "world_manifolds",
            "Model", "State",
            "WorldDef", "GAME_DT", "STATIC", "KINEMATIC", "DYNAMIC", "REVOLUTE", "PRISMATIC", "WELD", "compact_model",
-           "compact_state", "expand_state", "debug", "io", "layout", "record", "scenes", "shapes", "world"]
+           "compact_state", "expand_state", "debug", "io", "layout", "policy", "record", "scenes", "shapes", "world"]

@@ -76,9 +76,23 @@ class GoiLaunchInfo(ctypes.Structure):
 
 KERNEL_GENERIC, KERNEL_RIG, KERNEL_ISLAND, KERNEL_COLLIDE = 1, 2, 3, 4  # GOI_KERNEL_*
 
+F32, F16, BF16 = 0, 1, 2  # GOI_F32, GOI_F16, GOI_BF16 (include/goi_policy.h)
+_I64x3 = ctypes.c_int64 * 3
+
+
+class GoiAttention(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_worlds", "q_steps", "k_steps", "heads", "kv_heads", "dim", "type", "causal")] + [
+        ("scale", ctypes.c_float), ("n_buckets", ctypes.c_int32), ("n_distances", ctypes.c_int32),
+        ("bias_type", ctypes.c_int32), ("q", _P), ("k", _P), ("v", _P), ("q_strides", _I64x3), ("k_strides", _I64x3),
+        ("v_strides", _I64x3), ("bias", _P), ("buckets", _P), ("first", _P), ("lengths", _P), ("out", _P),
+        ("out_strides", _I64x3), ("stats", _P), ("dout", _P), ("dout_strides", _I64x3), ("dq", _P), ("dk", _P), ("dv", _P),
+        ("dq_strides", _I64x3), ("dk_strides", _I64x3), ("dv_strides", _I64x3), ("dbias", _P)]
+
+
 EXPORTS = ("goi_abi_version", "goi_model_create", "goi_model_destroy", "goi_step", "goi_step_n", "goi_step_n_noalloc",
            "goi_collide", "goi_world_manifold", "goi_apply_motor_actions", "goi_sincos", "goi_packed_layout",
            "goi_model_release_rows", "goi_last_launch", "goi_last_error")
+POLICY_EXPORTS = ("goi_attention_workspace", "goi_attention_forward", "goi_attention_backward")
 
 _LIB = None
 
@@ -122,6 +136,12 @@ def lib(path=None):
     L.goi_model_release_rows.restype = ctypes.c_int32
     L.goi_last_launch.argtypes = [ctypes.POINTER(GoiLaunchInfo)]
     L.goi_last_launch.restype = ctypes.c_int32
+    att = ctypes.POINTER(GoiAttention)
+    L.goi_attention_workspace.argtypes = [att, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
+    L.goi_attention_forward.argtypes = [att, _P, ctypes.c_uint64, _P]
+    L.goi_attention_backward.argtypes = [att, _P, ctypes.c_uint64, _P]
+    for name in POLICY_EXPORTS:
+        getattr(L, name).restype = ctypes.c_int32
     if L.goi_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{p}: ABI version {L.goi_abi_version()} != {ABI_VERSION}")
     if path is None:

@@ -374,6 +374,13 @@ struct WideBuild {
 
 }  // namespace
 
+namespace goi {
+
+// goi_last_error()'s text, for the library's other translation units (policy.hpp)
+int set_error(int code, const char* msg) { return fail(code, msg); }
+
+}  // namespace goi
+
 extern "C" {
 
 int32_t goi_abi_version(void) { return GOI_ABI_VERSION; }

@@ -1,0 +1,134 @@
+// policy.hpp - what the policy operators' kernels share: element types, the matrix instructions, 16-bit tiles in LDS and
+// the error text of a failed call.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/goi_b2.h"
+#include "../../include/goi_policy.h"
+
+// the operators' sums are ordinary float arithmetic: products and additions may be fused (the step's files forbid it)
+#pragma clang fp contract(fast)
+
+namespace goi {
+
+// Sets goi_last_error()'s text and returns code (goi_b2.hip).
+int set_error(int code, const char* msg);
+
+inline int policy_error(int code, const char* fmt, ...) {
+    char msg[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(msg, sizeof msg, fmt, ap);
+    va_end(ap);
+    return set_error(code, msg);
+}
+
+inline int launch_error(const char* who) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GOI_OK : policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
+}
+
+using bf16 = __bf16;
+using f16 = _Float16;
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Half;  // the 16-bit types' vectors
+template <> struct Half<bf16> { using x4 = bf16x4; using x8 = bf16x8; };
+template <> struct Half<f16> { using x4 = f16x4; using x8 = f16x8; };
+template <typename T> using half4 = typename Half<T>::x4;
+template <typename T> using half8 = typename Half<T>::x8;
+
+// c + a b on 32 x 32 x 16. Lane l holds a[l & 31][8 * (l >> 5) ..+7] and b[8 * (l >> 5) ..+7][l & 31]; of c, column l & 31
+// and rows (r & 3) + 8 * (r >> 2) + 4 * (l >> 5), r = 0 .. 15.
+__device__ __forceinline__ float16_t mfma(bf16x8 a, bf16x8 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16_t mfma(f16x8 a, f16x8 b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ int mfma_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// the value of the lane 32 away
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+__device__ __forceinline__ int wave_min(int x) {
+    for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int wave_max(int x) {
+    for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// Block b's place in a grid of nb blocks so that each of the 8 XCDs (block b runs on XCD b % 8, each with its own L2) takes
+// one contiguous range of places: a bijection for any nb.
+__device__ __forceinline__ int xcd_place(int b, int nb) {
+    const int x = b & 7, q = nb >> 3, r = nb & 7;
+    return x * q + min(x, r) + (b >> 3);
+}
+
+// A tile of 16-bit rows of DP elements in LDS, in chunks of 8 elements (16 bytes). Chunk ch of row `row` sits at
+// chunk_at(row, ch): exclusive-or with bits of the row spreads over the 64 banks both the reads down a column of chunks
+// (16 rows, one chunk) and the transposing reads (4 consecutive rows, 4 chunks each). It depends on row % 16 only.
+template <int DP>
+__device__ __forceinline__ int chunk_at(int row, int ch) {
+    static_assert(DP == 32 || DP == 64 || DP == 128, "row lengths with a layout");
+    int f;
+    if constexpr (DP == 32) f = (row >> 2) & 3;
+    else if constexpr (DP == 64) f = ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    else f = (row & 3) << 2 | ((row >> 2) & 3);
+    return row * (DP / 8) + (ch ^ f);
+}
+
+// a[l & 31][8 (l >> 5) ..] of mfma's first operand: rows row0 .. row0 + 31 of the tile, columns 16 s .. 16 s + 15
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> row_fragment(const T* tile, int row0, int s, int lane) {
+    return reinterpret_cast<const half8<T>*>(tile)[chunk_at<DP>(row0 + (lane & 31), 2 * s + (lane >> 5))];
+}
+
+// The first operand of a product over the tile's ROWS: a[d][k] = tile[row0 + k'][d0 + d], d = 0 .. 31, where k' runs over
+// row0's 16 rows in the order in which a float16_t of mfma holds them (mfma_row: registers 8 x .. 8 x + 7 of a lane, x = row0 / 16 of
+// the block), so that such registers, rounded, are the second operand as they stand. The transposing read gives lane i of
+// each 16 lanes element i of four rows, each row's 16 elements addressed by four of the lanes, 8 bytes each.
+template <typename T, int DP>
+__device__ __forceinline__ half8<T> column_fragment(const T* tile, int row0, int d0, int lane) {
+    typedef short4_t __attribute__((address_space(3))) * LdsPtr;
+    union {
+        short4_t part[2];
+        half8<T> all;
+    } u;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int row = row0 + 8 * t + 4 * (lane >> 5) + ((lane & 15) >> 2);
+        const int col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const T* p = tile + chunk_at<DP>(row, col >> 3) * 8 + (col & 4);
+        u.part[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
+    }
+    return u.all;
+}
+
+// registers 8 x .. 8 x + 7 of a product as the second operand of the next one (see column_fragment)
+template <typename T>
+__device__ __forceinline__ half8<T> to_operand(const float16_t& c, int x) {
+    float8_t f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = c[8 * x + e];
+    return __builtin_convertvector(f, half8<T>);
+}
+
+}  // namespace goi

@@ -1,0 +1,442 @@
+// policy_attention.hip - attention over the worlds' histories: the forward kernels and the C entry points
+// (include/goi_policy.h). One pass over the keys with the running maximum and sum of the softmax.
+#include <algorithm>
+
+#include "policy_attention.hpp"
+
+namespace goi {
+namespace {
+
+// NW waves of 32 packed rows each share tiles of KT keys. Two tiles of LDS (one for a single wave, which needs no barrier):
+// the next tile's loads are in flight while this one is computed.
+template <typename T, int DP, int NW, bool kSplit>
+__global__ void __launch_bounds__(64 * NW) k_attention(const AttnRun A) {
+    constexpr int NT = 64 * NW, KT = NW == 1 && DP == 128 ? 32 : 64, KB = KT / 32, NBUF = NW == 1 ? 1 : 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ int range[2][NW];
+    T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][keys, values][KT][DP]
+    float* const table = reinterpret_cast<float*>(lds + NBUF * 2 * KT * DP * sizeof(T));
+    const GoiAttention& a = A.a;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+
+    int place = xcd_place(blockIdx.x, gridDim.x);
+    // the later row tiles of a causal window see the most keys: they go first
+    const int tile = A.tiles - 1 - place % A.tiles;
+    place /= A.tiles;
+    const int split = kSplit ? place % A.splits : 0;
+    if (kSplit) place /= A.splits;
+    const int n = place / a.kv_heads, g = place - n * a.kv_heads;
+
+    const int L = history(A, n), m = (tile * NW + wave) * 32 + (lane & 31);
+    Row row = make_row(A, n, L, m);
+    if (kSplit) {
+        row.lo = max(row.lo, split * A.span);
+        row.hi = min(row.hi, (split + 1) * A.span);
+        if (row.hi <= row.lo) row.lo = row.hi = 0;
+    }
+    const BlockInfo blk = make_block(row);
+    if (lane == 0) {
+        range[0][wave] = blk.lo;
+        range[1][wave] = blk.hi;
+    }
+    const float* bias = nullptr;
+    if (a.bias) {
+        stage_bias(A, g, table, tid, NT);
+        bias = table + row.hl * a.n_distances;
+    }
+    const int head = g * A.group + row.hl;
+    half8<T> q[DP / 16];
+    load_operand<T, DP>(q, static_cast<const T*>(a.q) + n * a.q_strides[0] + row.i * a.q_strides[1] + head * a.q_strides[2],
+                        row.valid, a.dim, lane);
+    __syncthreads();
+    int lo = INT_MAX, hi = 0;  // the keys that some row of the block sees
+    for (int w = 0; w < NW; ++w) {
+        lo = min(lo, range[0][w]);
+        hi = max(hi, range[1][w]);
+    }
+
+    float16_t o[DP / 32];
+    clear(o);
+    float top = -INFINITY, sum = 0.0f;
+    if (lo < hi) {
+        const T* const kp = static_cast<const T*>(a.k) + n * a.k_strides[0] + g * a.k_strides[2];
+        const T* const vp = static_cast<const T*>(a.v) + n * a.v_strides[0] + g * a.v_strides[2];
+        KeyStage<T, DP, KT, NT> ks, vs;
+        ks.load(kp, a.k_strides[1], lo, lo, hi, a.dim, tid);
+        vs.load(vp, a.v_strides[1], lo, lo, hi, a.dim, tid);
+        ks.store(tiles, lo, lo, hi, a.dim, tid);
+        vs.store(tiles + KT * DP, lo, lo, hi, a.dim, tid);
+        __syncthreads();
+        int buf = 0;
+        for (int k0 = lo; k0 < hi; k0 += KT) {
+            const bool more = k0 + KT < hi;
+            if (more) {
+                ks.load(kp, a.k_strides[1], k0 + KT, lo, hi, a.dim, tid);
+                vs.load(vp, a.v_strides[1], k0 + KT, lo, hi, a.dim, tid);
+            }
+            const T* const kt = tiles + buf * 2 * KT * DP;
+            const T* const vt = kt + KT * DP;
+            if (k0 < blk.hi && k0 + KT > blk.lo) {
+                float16_t s[KB];
+                float best = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+                    const int key0 = k0 + 32 * b;
+                    s[b] = raw_scores<T, DP>(kt, 32 * b, q, lane);
+                    scale_scores(s[b], A.c, bias, a.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
+                    if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = key0 + mfma_row(r, half);
+                            s[b][r] = key >= row.lo && key < row.hi ? s[b][r] : -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
+                }
+                best = fmaxf(best, other_half(best));
+                if (__any(best > top)) {
+                    const float next = fmaxf(top, best);
+                    const float f = next == -INFINITY ? 1.0f : exp2_fast(top - next);
+                    top = next;
+                    sum *= f;
+#pragma unroll
+                    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[b][r] *= f;
+                }
+                const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        s[b][r] = exp2_fast(s[b][r] - base);
+                        sum += s[b][r];
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const half8<T> p = to_operand<T>(s[b], x);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d)
+                            o[d] = mfma(column_fragment<T, DP>(vt, 32 * b + 16 * x, 32 * d, lane), p, o[d]);
+                    }
+                }
+            }
+            if (NBUF == 1) __syncthreads();
+            else buf ^= 1;
+            if (more) {
+                ks.store(tiles + buf * 2 * KT * DP, k0 + KT, lo, hi, a.dim, tid);
+                vs.store(tiles + buf * 2 * KT * DP + KT * DP, k0 + KT, lo, hi, a.dim, tid);
+            }
+            __syncthreads();
+        }
+    }
+    sum += other_half(sum);
+    if (!row.valid) return;
+    if (kSplit) {
+        const int64_t at = ((int64_t)split * a.n_worlds * a.kv_heads + n * a.kv_heads + g) * A.rows + m;
+        if (half == 0) A.part_ml[at] = make_float2(top, sum);
+        float* const to = A.part_o + at * a.dim;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 32 * b + 8 * x + 4 * half;
+                if (d < a.dim)
+                    *reinterpret_cast<float4_t*>(to + d) =
+                        float4_t{o[b][4 * x], o[b][4 * x + 1], o[b][4 * x + 2], o[b][4 * x + 3]};
+            }
+        return;
+    }
+    T* const to = static_cast<T*>(a.out) + n * a.out_strides[0] + row.i * a.out_strides[1] + head * a.out_strides[2];
+    store_row<T, DP>(to, o, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, a.dim, half);
+    if (a.stats && half == 0)
+        reinterpret_cast<float2*>(a.stats)[((int64_t)n * a.heads + head) * a.q_steps + row.i] = make_float2(top, sum);
+}
+
+// Joins the splits of each row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, M the largest m_s. A wave a row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
+    const GoiAttention& a = A.a;
+    const int64_t rows = (int64_t)a.n_worlds * a.kv_heads * A.rows;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int s = lane; s < A.splits; s += 64) top = fmaxf(top, A.part_ml[s * rows + row].x);
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, x = 0.0f, y = 0.0f;
+    const bool in = 2 * lane < a.dim;
+    for (int s = 0; s < A.splits; ++s) {
+        const float2 ml = A.part_ml[s * rows + row];
+        const float f = exp2_fast(ml.x - base);
+        sum += f * ml.y;
+        if (in) {
+            const float2 o = *reinterpret_cast<const float2*>(A.part_o + (s * rows + row) * a.dim + 2 * lane);
+            x += f * o.x;
+            y += f * o.y;
+        }
+    }
+    const int64_t pair = row / A.rows;
+    const int m = (int)(row - pair * A.rows), i = m / A.group;
+    const int n = (int)(pair / a.kv_heads), head = (int)(pair - (int64_t)n * a.kv_heads) * A.group + m - i * A.group;
+    const float f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    T* const to = static_cast<T*>(a.out) + n * a.out_strides[0] + i * a.out_strides[1] + head * a.out_strides[2];
+    if (in) {
+        to[2 * lane] = (T)(x * f);
+        to[2 * lane + 1] = (T)(y * f);
+    }
+    if (a.stats && lane == 0)
+        reinterpret_cast<float2*>(a.stats)[((int64_t)n * a.heads + head) * a.q_steps + i] = make_float2(top, sum);
+}
+
+// dbias from the row tiles' parts [count][columns]: block (x, y) sums rows y, y + gridDim.y, ... of 64 columns, then the
+// second launch (one row of blocks) the sums. Fixed order.
+__global__ void __launch_bounds__(256) k_bias_sum(const float* parts, int count, int columns, float* sums, void* out, int type) {
+    __shared__ float part[4][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
+    float s = 0.0f;
+    if (col < columns)
+        for (int64_t r = (int64_t)blockIdx.y * 4 + sub; r < count; r += (int64_t)gridDim.y * 4) s += parts[r * columns + col];
+    part[sub][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (sub || col >= columns) return;
+    s = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    if (sums) sums[(int64_t)blockIdx.y * columns + col] = s;
+    else if (type == GOI_F32) static_cast<float*>(out)[col] = s;
+    else if (type == GOI_F16) static_cast<f16*>(out)[col] = (f16)s;
+    else static_cast<bf16*>(out)[col] = (bf16)s;
+}
+
+// ---------------------------------------------------------------- host
+
+bool aligned(const void* p, const int64_t* strides) {
+    return p && ((uintptr_t)p & 15) == 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0;
+}
+
+constexpr int kWavesWanted = 2048;  // waves that fill the chip: 256 CUs x 4 SIMDs x 2
+
+// Waves of 32 rows a block: enough for the rows of a key head, up to 4
+int waves_for(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+int check_sizes(const GoiAttention* a, AttnRun* A, const char* who) {
+    if (!a) return policy_error(GOI_E_ARG, "%s: null argument", who);
+    if (a->n_worlds < 0 || a->q_steps < 0 || a->k_steps < 0 || a->heads <= 0 || a->kv_heads <= 0)
+        return policy_error(GOI_E_ARG, "%s: negative sizes or no heads", who);
+    if (a->heads % a->kv_heads) return policy_error(GOI_E_SHAPE, "%s: heads is no multiple of kv_heads", who);
+    if (a->type != GOI_BF16 && a->type != GOI_F16) return policy_error(GOI_E_UNSUPPORTED, "%s: type is neither bf16 nor f16", who);
+    if (a->dim < 8 || a->dim > 128 || a->dim % 8)
+        return policy_error(GOI_E_UNSUPPORTED, "%s: dim %d is no multiple of 8 within 8 .. 128", who, a->dim);
+    A->a = *a;
+    A->group = a->heads / a->kv_heads;
+    const int64_t rows = (int64_t)a->q_steps * A->group;
+    if (rows > INT_MAX - 256 || a->k_steps > INT_MAX - 256 || (int64_t)a->n_worlds * a->heads > INT_MAX)
+        return policy_error(GOI_E_UNSUPPORTED, "%s: sizes above 31 bits", who);
+    if (a->bias) {
+        if (!a->buckets) return policy_error(GOI_E_ARG, "%s: a bias without buckets", who);
+        if (a->n_buckets < 1 || a->n_distances < 1) return policy_error(GOI_E_ARG, "%s: an empty bias", who);
+        if (a->bias_type != a->type && a->bias_type != GOI_F32)
+            return policy_error(GOI_E_UNSUPPORTED, "%s: the bias is of another 16-bit type", who);
+        if (!a->causal && a->n_distances % 2 == 0)
+            return policy_error(GOI_E_SHAPE, "%s: without a causal order buckets holds both directions and distance 0", who);
+        if (a->n_buckets > kMaxBuckets || (int64_t)A->group * a->n_distances > kMaxBiasTable)
+            return policy_error(GOI_E_UNSUPPORTED, "%s: more than %d buckets, or group * n_distances above %d", who, kMaxBuckets,
+                                kMaxBiasTable);
+    }
+    A->rows = (int)rows;
+    A->blocks = (A->rows + 31) / 32;
+    A->origin = a->causal ? 0 : (a->n_distances - 1) / 2;
+    A->c = a->scale * kLog2e;
+    A->splits = 1;
+    A->span = 0;
+    A->part_o = nullptr;
+    A->part_ml = nullptr;
+    A->row_info = nullptr;
+    A->block_info = nullptr;
+    A->part_bias = nullptr;
+    return GOI_OK;
+}
+
+int check_grid(int64_t blocks, const char* who) {
+    return blocks > INT_MAX ? policy_error(GOI_E_UNSUPPORTED, "%s: more than 2^31 blocks", who) : GOI_OK;
+}
+
+// The key axis is split where the row tiles alone would leave the chip mostly idle: into as many ranges of at least 128 keys
+// as bring the waves to kWavesWanted.
+void plan_forward(AttnRun* A, int* waves) {
+    const GoiAttention& a = A->a;
+    *waves = waves_for(A->rows);
+    A->tiles = (A->rows + 32 * *waves - 1) / (32 * *waves);
+    const int64_t blocks = (int64_t)a.n_worlds * a.kv_heads * A->tiles;
+    const int64_t want = kWavesWanted / std::max<int64_t>(1, blocks * *waves);
+    const int64_t most = (a.k_steps + 127) / 128;
+    A->splits = (int)std::max<int64_t>(1, std::min(want, most));
+    A->span = ((a.k_steps + A->splits - 1) / A->splits + 63) / 64 * 64;
+    if (A->span > 0) A->splits = (a.k_steps + A->span - 1) / A->span;
+    A->splits = std::max(A->splits, 1);
+}
+
+uint64_t round16(uint64_t x) { return (x + 15) & ~(uint64_t)15; }
+
+uint64_t forward_bytes(const AttnRun& A) {
+    if (A.splits <= 1) return 0;
+    const uint64_t rows = (uint64_t)A.a.n_worlds * A.a.kv_heads * A.rows * A.splits;
+    return round16(rows * sizeof(float2)) + rows * A.a.dim * sizeof(float);
+}
+
+// The backward scratch: row and block infos, dbias' parts and their first sums.
+constexpr int kBiasSums = 128;
+struct BackwardPlan {
+    int waves, tiles;
+    uint64_t blocks_at, parts_at, sums_at, bytes;
+    int64_t parts;
+};
+BackwardPlan plan_backward(const AttnRun& A) {
+    BackwardPlan p;
+    const GoiAttention& a = A.a;
+    p.waves = waves_for(A.rows);
+    p.tiles = (A.rows + 32 * p.waves - 1) / (32 * p.waves);
+    const uint64_t pairs = (uint64_t)a.n_worlds * a.kv_heads;
+    p.blocks_at = round16(pairs * A.rows * sizeof(RowInfo));
+    p.parts_at = round16(p.blocks_at + pairs * A.blocks * sizeof(BlockInfo));
+    p.parts = (int64_t)a.n_worlds * p.tiles;
+    const uint64_t columns = a.bias ? (uint64_t)a.heads * a.n_buckets : 0;
+    p.sums_at = round16(p.parts_at + p.parts * columns * sizeof(float));
+    p.bytes = p.sums_at + kBiasSums * columns * sizeof(float);
+    return p;
+}
+
+template <typename T, int DP, int NW>
+hipError_t launch_forward(const AttnRun& A, hipStream_t st) {
+    constexpr int KT = NW == 1 && DP == 128 ? 32 : 64, NBUF = NW == 1 ? 1 : 2;
+    const size_t lds = NBUF * 2 * KT * DP * sizeof(T) + (A.a.bias ? (size_t)A.group * A.a.n_distances * sizeof(float) : 0);
+    const dim3 grid((unsigned)((int64_t)A.a.n_worlds * A.a.kv_heads * A.tiles * A.splits)), block(64 * NW);
+    if (A.splits > 1) {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention<T, DP, NW, true>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL((k_attention<T, DP, NW, true>), grid, block, lds, st, A);
+        const int64_t rows = (int64_t)A.a.n_worlds * A.a.kv_heads * A.rows;
+        hipLaunchKernelGGL(k_attention_join<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, A);
+    } else {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention<T, DP, NW, false>),
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL((k_attention<T, DP, NW, false>), grid, block, lds, st, A);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, int DP>
+hipError_t launch_forward(const AttnRun& A, int waves, hipStream_t st) {
+    return waves == 1 ? launch_forward<T, DP, 1>(A, st) : waves == 2 ? launch_forward<T, DP, 2>(A, st)
+                                                                     : launch_forward<T, DP, 4>(A, st);
+}
+
+template <typename T>
+hipError_t launch_forward(const AttnRun& A, int waves, hipStream_t st) {
+    const int dp = attention_dim_tile(A.a.dim);
+    return dp == 32 ? launch_forward<T, 32>(A, waves, st) : dp == 64 ? launch_forward<T, 64>(A, waves, st)
+                                                                    : launch_forward<T, 128>(A, waves, st);
+}
+
+}  // namespace
+
+int attention_dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+}  // namespace goi
+
+using namespace goi;
+
+extern "C" {
+
+int32_t goi_attention_workspace(const GoiAttention* a, int32_t backward, uint64_t* bytes) {
+    AttnRun A;
+    if (!bytes) return policy_error(GOI_E_ARG, "goi_attention_workspace: null argument");
+    const int rc = check_sizes(a, &A, "goi_attention_workspace");
+    if (rc != GOI_OK) return rc;
+    if (backward) {
+        *bytes = plan_backward(A).bytes;
+    } else {
+        int waves;
+        plan_forward(&A, &waves);
+        *bytes = forward_bytes(A);
+    }
+    return GOI_OK;
+}
+
+int32_t goi_attention_forward(const GoiAttention* a, void* workspace, uint64_t workspace_bytes, void* hip_stream) {
+    const char* const who = "goi_attention_forward";
+    AttnRun A;
+    int rc = check_sizes(a, &A, who);
+    if (rc != GOI_OK) return rc;
+    if (a->n_worlds == 0 || a->q_steps == 0) return GOI_OK;
+    if (!aligned(a->q, a->q_strides) || !aligned(a->out, a->out_strides) ||
+        (a->k_steps > 0 && (!aligned(a->k, a->k_strides) || !aligned(a->v, a->v_strides))))
+        return policy_error(GOI_E_ARG, "%s: a null or misaligned tensor (16-byte pointers, strides of 8 elements)", who);
+    int waves;
+    plan_forward(&A, &waves);
+    if (forward_bytes(A) > workspace_bytes || (forward_bytes(A) && (!workspace || (uintptr_t)workspace & 15)))
+        return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
+    rc = check_grid((int64_t)a->n_worlds * a->kv_heads * A.tiles * A.splits, who);
+    if (rc != GOI_OK) return rc;
+    if (A.splits > 1) {
+        const uint64_t rows = (uint64_t)a->n_worlds * a->kv_heads * A.rows * A.splits;
+        A.part_ml = static_cast<float2*>(workspace);
+        A.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + round16(rows * sizeof(float2)));
+    }
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const hipError_t e = a->type == GOI_BF16 ? launch_forward<bf16>(A, waves, st) : launch_forward<f16>(A, waves, st);
+    if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
+    return GOI_OK;
+}
+
+int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t workspace_bytes, void* hip_stream) {
+    const char* const who = "goi_attention_backward";
+    AttnRun A;
+    int rc = check_sizes(a, &A, who);
+    if (rc != GOI_OK) return rc;
+    if (a->bias && !a->dbias) return policy_error(GOI_E_ARG, "%s: null dbias", who);
+    const bool rows = a->n_worlds > 0 && a->q_steps > 0, keys = a->n_worlds > 0 && a->k_steps > 0;
+    if ((rows && (!aligned(a->q, a->q_strides) || !aligned(a->out, a->out_strides) || !aligned(a->dout, a->dout_strides) ||
+                  !aligned(a->dq, a->dq_strides) || !a->stats || (uintptr_t)a->stats & 7)) ||
+        (keys && (!aligned(a->k, a->k_strides) || !aligned(a->v, a->v_strides) || !aligned(a->dk, a->dk_strides) ||
+                  !aligned(a->dv, a->dv_strides))))
+        return policy_error(GOI_E_ARG, "%s: a null or misaligned tensor (16-byte pointers, strides of 8 elements)", who);
+    const BackwardPlan p = plan_backward(A);
+    if (p.bytes > workspace_bytes || (p.bytes && (!workspace || (uintptr_t)workspace & 15)))
+        return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
+    const int64_t pairs = (int64_t)a->n_worlds * a->kv_heads;
+    rc = check_grid(pairs * std::max<int64_t>(p.tiles, (a->k_steps + 31) / 32), who);
+    if (rc != GOI_OK) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    char* const ws = static_cast<char*>(workspace);
+    A.row_info = reinterpret_cast<RowInfo*>(ws);
+    A.block_info = reinterpret_cast<BlockInfo*>(ws + p.blocks_at);
+    A.part_bias = reinterpret_cast<float*>(ws + p.parts_at);
+    A.tiles = p.tiles;
+    hipError_t e = hipSuccess;
+    if (rows) e = launch_attention_dq(A, p.waves, st);
+    if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
+    if (a->bias) {
+        const int columns = a->heads * a->n_buckets, x = (columns + 63) / 64;
+        float* const sums = reinterpret_cast<float*>(ws + p.sums_at);
+        const int count = rows ? (int)p.parts : 0, y = std::max(1, std::min(kBiasSums, (count + 3) / 4));
+        if (y > 1)
+            hipLaunchKernelGGL(k_bias_sum, dim3(x, y), dim3(256), 0, st, A.part_bias, count, columns, sums, nullptr, 0);
+        hipLaunchKernelGGL(k_bias_sum, dim3(x, 1), dim3(256), 0, st, y > 1 ? sums : A.part_bias, y > 1 ? y : count, columns,
+                           nullptr, a->dbias, a->bias_type);
+        rc = launch_error(who);
+        if (rc != GOI_OK) return rc;
+    }
+    if (keys) {
+        // keys of 32 a wave: fewer waves a block where blocks of 4 would not fill the chip
+        int waves = waves_for(a->k_steps);
+        while (waves > 1 && pairs * ((a->k_steps + 32 * waves - 1) / (32 * waves)) < 512) waves /= 2;
+        A.tiles = (a->k_steps + 32 * waves - 1) / (32 * waves);
+        e = launch_attention_dkv(A, waves, st);
+        if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
+    }
+    return GOI_OK;
+}
+
+}  // extern "C"

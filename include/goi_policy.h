@@ -1,0 +1,84 @@
+/* goi_policy.h - C ABI of the policy operators of libgoi_b2.so: what a policy network over the worlds' histories runs on
+ * the GPU between two steps of goi_b2.h, in training and in acting. No counterpart in the reference's physics package, whose
+ * callers bring their own networks.
+ *
+ * Conventions are goi_b2.h's: int return codes (GOI_OK, GOI_E_ARG, GOI_E_SHAPE, GOI_E_HIP, GOI_E_UNSUPPORTED) with
+ * goi_last_error(); calls are asynchronous on the given hipStream_t; every buffer is device memory of the caller. Nothing here
+ * allocates, keeps state between calls or synchronises: where an operator needs scratch memory, goi_*_workspace says how many
+ * bytes, and the caller passes a buffer (16-byte aligned, any contents) that no other call uses until this one has run. All
+ * calls can be captured into a HIP graph. Results do not depend on timing: no sum is taken by atomics whose order varies.
+ * Empty batches are GOI_OK and launch nothing, or write the zeros that an empty sum is.
+ */
+#ifndef GOI_POLICY_H
+#define GOI_POLICY_H
+
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element types. */
+#define GOI_F32 0
+#define GOI_F16 1
+#define GOI_BF16 2
+
+/* Attention of each world's steps over its history, with key heads shared by groups of query heads, a learned bias by
+ * distance, episodes inside a window and ragged caches.
+ *
+ *   q [n_worlds, q_steps, heads, dim], k and v [n_worlds, k_steps, kv_heads, dim], out like q; heads = kv_heads * group, query head
+ *   h reads key head h / group. With L = lengths[w] clamped to 0 .. k_steps (k_steps where lengths is null), the queries are the
+ *   last q_steps of the L positions: query i stands at p = L - q_steps + i. It sees the keys j with
+ *       max(0, first[w, i]) <= j < (causal ? min(p + 1, L) : L)
+ *   (first may be null: 0), scores them
+ *       s = scale * q.k + bias[h, buckets[clamp(p - j + o, 0, n_distances - 1)]]
+ *   with o = 0 for causal and (n_distances - 1) / 2 otherwise (bias may be null: no bias), and
+ *       out = sum_j softmax(s)_j v_j,     stats = { M, sum_j 2^(s_j log2(e) - M) } with M = max_j s_j log2(e)
+ *   (two numbers and not the logarithm of the sum, which would lose the sum where M is a mask's -3e38). A query that sees
+ *   no key, or only scores of minus infinity, gives out = 0 and stats = { minus infinity, 0 }, and no gradient.
+ *   Keys and values that no query sees may hold anything, NaN and infinities among them, and are not read past L.
+ *
+ * Products are of the 16-bit inputs with float32 sums; the maximum, the sum and the accumulators of the softmax are float32;
+ * probabilities and their gradients are rounded to the inputs' type for the second products.
+ *
+ * Limits: type GOI_BF16 or GOI_F16; dim a multiple of 8, 8 .. 128; 16-byte aligned pointers and strides (elements) that are
+ * multiples of 8, the last axis contiguous; n_buckets <= 64; group * n_distances <= 4096. A bucket outside 0 .. n_buckets - 1 is
+ * taken as the nearest one. bias_type is type or GOI_F32. stats is [n_worlds, heads, q_steps, 2] contiguous and may be null in the
+ * forward call. */
+typedef struct GoiAttention {
+    int32_t n_worlds, q_steps, k_steps, heads, kv_heads, dim;
+    int32_t type;   /* GOI_BF16 or GOI_F16: q, k, v, out and their gradients */
+    int32_t causal; /* 0 or 1 */
+    float scale;
+    int32_t n_buckets, n_distances, bias_type;
+    const void *q, *k, *v;
+    int64_t q_strides[3], k_strides[3], v_strides[3]; /* world, step, head */
+    const void* bias;       /* [heads, n_buckets] contiguous, or null */
+    const int32_t* buckets; /* [n_distances] (required with bias) */
+    const int32_t* first;   /* [n_worlds, q_steps] contiguous, or null */
+    const int32_t* lengths; /* [n_worlds], or null */
+    void* out;
+    int64_t out_strides[3];
+    float* stats;
+    /* goi_attention_backward only: the gradient of out, and the gradients it writes (out and stats are its inputs) */
+    const void* dout;
+    int64_t dout_strides[3];
+    void *dq, *dk, *dv;
+    int64_t dq_strides[3], dk_strides[3], dv_strides[3];
+    void* dbias; /* [heads, n_buckets] contiguous, of bias_type; required with bias */
+} GoiAttention;
+
+/* Scratch bytes of goi_attention_forward (backward = 0) or goi_attention_backward (1) for these sizes (pointers other than
+ * bias and lengths are not looked at). */
+int32_t goi_attention_workspace(const GoiAttention* a, int32_t backward, uint64_t* bytes);
+
+int32_t goi_attention_forward(const GoiAttention* a, void* workspace, uint64_t workspace_bytes, void* hip_stream);
+
+/* The gradients of q, k, v and bias from dout, out and stats; the probabilities are computed again from q, k and stats. */
+int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t workspace_bytes, void* hip_stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* GOI_POLICY_H */
