@@ -89,10 +89,32 @@ class GoiAttention(ctypes.Structure):
         ("dq_strides", _I64x3), ("dk_strides", _I64x3), ("dv_strides", _I64x3), ("dbias", _P)]
 
 
+class GoiNorm(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("width", ctypes.c_int32), ("type", ctypes.c_int32), ("weight_type", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("x", _P), ("x_stride", ctypes.c_int64), ("residual", _P),
+                ("residual_stride", ctypes.c_int64), ("weight", _P), ("r", _P), ("r_stride", ctypes.c_int64), ("y", _P),
+                ("y_stride", ctypes.c_int64), ("values", _P), ("values_stride", ctypes.c_int64), ("scales", _P), ("inv", _P)]
+
+
+class GoiNormBackward(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("width", ctypes.c_int32), ("type", ctypes.c_int32), ("weight_type", ctypes.c_int32),
+                ("dy", _P), ("dy_stride", ctypes.c_int64), ("r", _P), ("r_stride", ctypes.c_int64), ("dresidual", _P),
+                ("dresidual_stride", ctypes.c_int64), ("weight", _P), ("inv", _P), ("dx", _P), ("dx_stride", ctypes.c_int64),
+                ("dweight", _P)]
+
+
+class GoiInt8(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("channels", ctypes.c_int32), ("width", ctypes.c_int32), ("type", ctypes.c_int32),
+                ("bias_type", ctypes.c_int32), ("x", _P), ("x_stride", ctypes.c_int64), ("x_scales", _P), ("w", _P),
+                ("w_stride", ctypes.c_int64), ("w_scales", _P), ("bias", _P), ("y", _P), ("y_stride", ctypes.c_int64)]
+
+
 EXPORTS = ("goi_abi_version", "goi_model_create", "goi_model_destroy", "goi_step", "goi_step_n", "goi_step_n_noalloc",
            "goi_collide", "goi_world_manifold", "goi_apply_motor_actions", "goi_sincos", "goi_packed_layout",
            "goi_model_release_rows", "goi_last_launch", "goi_last_error")
-POLICY_EXPORTS = ("goi_attention_workspace", "goi_attention_forward", "goi_attention_backward")
+POLICY_EXPORTS = ("goi_attention_workspace", "goi_attention_forward", "goi_attention_backward", "goi_rms_norm",
+                  "goi_rms_norm_backward_workspace", "goi_rms_norm_backward", "goi_linear_int8", "goi_clip_workspace",
+                  "goi_clip_gradients")
 
 _LIB = None
 
@@ -140,6 +162,12 @@ def lib(path=None):
     L.goi_attention_workspace.argtypes = [att, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
     L.goi_attention_forward.argtypes = [att, _P, ctypes.c_uint64, _P]
     L.goi_attention_backward.argtypes = [att, _P, ctypes.c_uint64, _P]
+    L.goi_rms_norm.argtypes = [ctypes.POINTER(GoiNorm), _P]
+    L.goi_rms_norm_backward_workspace.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
+    L.goi_rms_norm_backward.argtypes = [ctypes.POINTER(GoiNormBackward), _P, ctypes.c_uint64, _P]
+    L.goi_linear_int8.argtypes = [ctypes.POINTER(GoiInt8), _P]
+    L.goi_clip_workspace.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
+    L.goi_clip_gradients.argtypes = [ctypes.c_int32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, ctypes.c_uint64, _P]
     for name in POLICY_EXPORTS:
         getattr(L, name).restype = ctypes.c_int32
     if L.goi_abi_version() != ABI_VERSION:

@@ -3,6 +3,10 @@ steps of the worlds.
 
     out = policy.attention(q, k, v, bias=table, buckets=policy.distance_buckets(32, 128), first=episode_start)  # differentiable
     act = policy.attention(q1, k_cache, v_cache, bias=table, buckets=buckets, lengths=steps_held)                # one step
+    y, r = policy.rms_norm(x, gain, residual)                                                                    # differentiable
+    h, scale, r = policy.rms_norm_int8(x, gain, residual)
+    z = policy.linear_int8(h, scale, *policy.quantize_weight(w))
+    norm = policy.clip_gradients([p.grad for p in params], 0.5)
 
 Hand-written kernels for gfx950 through the C ABI in include/goi_policy.h; no fallback. Every call runs on the current
 stream of its tensors' device and waits for nothing. Tensors whose strides the kernels do not take (a last axis that is not
@@ -190,3 +194,211 @@ def attention(q, k, v, bias=None, buckets=None, first=None, lengths=None, causal
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
         return _Attention.apply(q, k, v, bias, buckets, first, lengths, causal, scale)
     return attention_forward(q, k, v, bias, buckets, first, lengths, causal, scale, need_stats=False)[0]
+
+
+# ---------------------------------------------------------------- norm
+
+
+def _flat(x, rows=None):
+    """x (..., width) as rows of contiguous elements (a view where its strides allow one)."""
+    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def _norm_args(x, weight, residual):
+    dev = _on_gpu(x, weight, residual)
+    _need(x.dtype in _TYPES and x.dim() >= 1, "x must be float32, float16 or bfloat16 with a last axis")
+    _need(weight.dtype in (x.dtype, torch.float32) and tuple(weight.shape) == x.shape[-1:],
+          "the weight is one row of x's type or float32")
+    _need(residual is None or (residual.dtype == x.dtype and residual.shape == x.shape), "the residual must be like x")
+    return dev, weight.contiguous()
+
+
+def _norm_call(x, weight, residual, eps, a, want_inv):
+    """Fills and runs GoiNorm (a holds y or values); returns (r, inv)."""
+    rows, width = x.shape[:-1].numel(), x.shape[-1]
+    a.rows, a.width, a.type, a.weight_type, a.eps = rows, width, _TYPES[x.dtype], _TYPES[weight.dtype], eps
+    x2 = _flat(x)
+    a.x, a.x_stride, a.weight = x2.data_ptr(), x2.stride(0), weight.data_ptr()
+    r = x
+    if residual is not None:
+        res = _flat(residual)
+        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        a.residual, a.residual_stride, a.r, a.r_stride = res.data_ptr(), res.stride(0), r.data_ptr(), width
+    inv = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_inv else None
+    a.inv = _ptr(inv)
+    L = _abi.lib()
+    with _guard(x.device):
+        _abi.check(L.goi_rms_norm(ctypes.byref(a), _stream(x.device)), L)
+    return r, inv
+
+
+def rms_norm_forward(x, weight, residual=None, eps=1e-6):
+    """(y, r, inv) of `rms_norm`, without a graph: r the residual stream (x itself without a residual), inv (...) float32 the
+    rows' 1 / sqrt(mean(r ** 2) + eps). rms_norm_backward needs r and inv."""
+    _, weight = _norm_args(x, weight, residual)
+    a = _abi.GoiNorm()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a.y, a.y_stride = y.data_ptr(), x.shape[-1]
+    r, inv = _norm_call(x, weight, residual, eps, a, True)
+    return y, r, inv
+
+
+def rms_norm_backward(dy, r, weight, inv, dresidual=None):
+    """(dx, dweight) of `rms_norm`: dx is the gradient of x and of the residual alike; dresidual is the gradient of r from where
+    it was used further on. dweight is of the weight's type, summed in float32 in a fixed order."""
+    dev, weight = _norm_args(r, weight, dresidual)
+    _on_gpu(r, dy, inv)
+    _need(dy.shape == r.shape and dy.dtype == r.dtype, "dy must be like r")
+    _need(inv.dtype == torch.float32 and inv.shape == r.shape[:-1], "inv must be rms_norm_forward's")
+    a = _abi.GoiNormBackward()
+    rows, width = r.shape[:-1].numel(), r.shape[-1]
+    a.rows, a.width, a.type, a.weight_type = rows, width, _TYPES[r.dtype], _TYPES[weight.dtype]
+    dx = torch.empty(r.shape, dtype=r.dtype, device=dev)
+    dweight = torch.empty_like(weight)
+    dy2, r2, inv = _flat(dy), _flat(r), inv.contiguous()
+    a.dy, a.dy_stride, a.r, a.r_stride = dy2.data_ptr(), dy2.stride(0), r2.data_ptr(), r2.stride(0)
+    if dresidual is not None:
+        dres = _flat(dresidual)
+        a.dresidual, a.dresidual_stride = dres.data_ptr(), dres.stride(0)
+    a.weight, a.inv, a.dx, a.dx_stride, a.dweight = weight.data_ptr(), inv.data_ptr(), dx.data_ptr(), width, dweight.data_ptr()
+    L = _abi.lib()
+    size = ctypes.c_uint64()
+    _abi.check(L.goi_rms_norm_backward_workspace(rows, width, ctypes.byref(size)), L)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        _abi.check(L.goi_rms_norm_backward(ctypes.byref(a), _ptr(ws), size.value, _stream(dev)), L)
+    return dx, dweight
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, r, inv = rms_norm_forward(x, weight, residual, eps)
+        ctx.save_for_backward(r, weight, inv)
+        ctx.added = residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, r) if ctx.added else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dr=None):
+        r, weight, inv = ctx.saved_tensors
+        if dy is None:
+            return dr, None, dr if ctx.added else None, None
+        dx, dweight = rms_norm_backward(dy, r, weight, inv, dr)
+        return dx, dweight, dx if ctx.added else None, None
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6):
+    """x / sqrt(mean(x ** 2) + eps) * weight over the last axis; with a residual of x + residual instead, and (y, x + residual) is
+    returned: the sum, rounded to x's type, is the residual stream for the next layer. Differentiable. float32, float16 or
+    bfloat16; weight of x's type or float32; float32 inside."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+        return _RmsNorm.apply(x, weight, residual, eps)
+    y, r, _ = rms_norm_forward(x, weight, residual, eps)
+    return y if residual is None else (y, r)
+
+
+# ---------------------------------------------------------------- 8-bit integers
+
+
+def rms_norm_int8(x, weight, residual=None, eps=1e-6):
+    """(values, scales, r): rms_norm's rows in 8 bits, values (..., width) int8 with scales (...) float32, the largest magnitude of
+    each row at 127, and the residual stream r (x itself without a residual). The input of `linear_int8`; rounded once,
+    from float32. A row with a value that is not finite has a scale of NaN. No gradient: for acting."""
+    dev, weight = _norm_args(x, weight, residual)
+    a = _abi.GoiNorm()
+    width = x.shape[-1]
+    pitch = (width + 15) // 16 * 16  # rows on 16 bytes, as linear_int8 reads them
+    values = torch.empty((*x.shape[:-1], pitch), dtype=torch.int8, device=dev)
+    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    a.values, a.values_stride, a.scales = values.data_ptr(), pitch, scales.data_ptr()
+    r, _ = _norm_call(x, weight, residual, eps, a, False)
+    return (values if pitch == width else values[..., :width]), scales, r
+
+
+def quantize_weight(weight):
+    """(values int8 (channels, width), scales float32 (channels,)) of a weight (channels, width): each channel's largest
+    magnitude at 127. Done once, with torch's own operations."""
+    _need(weight.dim() == 2, "a weight is (channels, width)")
+    w = weight.detach().float()
+    top = w.abs().amax(1) if w.shape[1] else w.new_zeros(w.shape[0])
+    scales = torch.where(top == 0, torch.ones_like(top), top / 127.0)
+    return (w / scales[:, None]).round().to(torch.int8), scales
+
+
+def _bytes16(x):
+    """int8 rows (r, width) as rows on 16 bytes, copied where they are not."""
+    if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (x.stride(0) % 16 == 0 or x.shape[0] == 1):
+        return x, x.stride(0) if x.shape[0] > 1 else 0
+    pitch = (x.shape[1] + 15) // 16 * 16
+    to = x.new_empty((x.shape[0], pitch))
+    to[:, :x.shape[1]].copy_(x)
+    return to, pitch
+
+
+def linear_int8(x, x_scales, weight, weight_scales, bias=None, dtype=torch.bfloat16):
+    """x_scales * weight_scales * (x @ weight.T) + bias: x (..., width) int8 with a scale a row (x_scales (...) float32), weight
+    (channels, width) int8 with a scale a channel; the sums are exact in 32 bits. bias (channels,) of dtype or float32. Returns
+    (..., channels) of dtype. No gradient: for acting."""
+    dev = _on_gpu(x, x_scales, weight, weight_scales, bias)
+    _need(x.dtype == torch.int8 and weight.dtype == torch.int8, "x and weight must be int8")
+    _need(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1], "x and weight must share their width")
+    _need(x_scales.dtype == torch.float32 and x_scales.shape == x.shape[:-1], "x_scales must be float32, one a row")
+    _need(weight_scales.dtype == torch.float32 and weight_scales.shape == weight.shape[:1],
+          "weight_scales must be float32, one a channel")
+    _need(dtype in _TYPES, "dtype must be float32, float16 or bfloat16")
+    _need(bias is None or (bias.dtype in (dtype, torch.float32) and bias.shape == weight.shape[:1]),
+          "the bias is one row of dtype or float32")
+    a = _abi.GoiInt8()
+    a.rows, a.channels, a.width, a.type = x.shape[:-1].numel(), weight.shape[0], weight.shape[1], _TYPES[dtype]
+    y = torch.empty((*x.shape[:-1], a.channels), dtype=dtype, device=dev)
+    x2, a.x_stride = _bytes16(x.flatten(0, -2) if x.dim() > 2 else x if x.dim() == 2 else x[None])
+    w2, a.w_stride = _bytes16(weight)
+    x_scales, weight_scales = x_scales.contiguous(), weight_scales.contiguous()
+    a.x, a.x_scales, a.w, a.w_scales = x2.data_ptr(), x_scales.data_ptr(), w2.data_ptr(), weight_scales.data_ptr()
+    if bias is not None:
+        bias = bias.contiguous()
+        a.bias, a.bias_type = bias.data_ptr(), _TYPES[bias.dtype]
+    a.y, a.y_stride = y.data_ptr(), a.channels
+    L = _abi.lib()
+    with _guard(dev):
+        _abi.check(L.goi_linear_int8(ctypes.byref(a), _stream(dev)), L)
+    return y
+
+
+# ---------------------------------------------------------------- gradients
+
+
+def clip_gradients(grads, max_norm, out=None):
+    """Clips gradients by their global norm: norm = sqrt(the sum of all their squares), every gradient times
+    min(1, max_norm / (norm + 1e-6)). In place, or into the tensors `out` (which may be of another of the three types, an
+    optimizer's float32 gradients say). Returns the norm before clipping, a float32 CUDA tensor: nothing waits for it. None among
+    the gradients is passed over, as a parameter without a gradient; a norm that is not finite gives what the formula
+    gives. Tensors must be contiguous; sums are taken in float64 in a fixed order."""
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    _need(len(outs) == len(grads), "as many outputs as gradients")
+    pairs = [(g, o) for g, o in zip(grads, outs) if g is not None]
+    if not pairs:
+        return torch.zeros((), device="cuda")
+    dev = pairs[0][0].device
+    for g, o in pairs:
+        if not (g.is_cuda and g.device == dev and o.device == dev and g.is_contiguous() and o.is_contiguous()
+                and g.dtype in _TYPES and o.dtype in _TYPES and g.shape == o.shape):
+            raise ValueError("gradients and outputs must be contiguous CUDA tensors of one device, float32, float16 or "
+                             "bfloat16, of equal shapes")
+    n = len(pairs)
+    pointers, longs, ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int32 * n
+    L = _abi.lib()
+    size = ctypes.c_uint64()
+    _abi.check(L.goi_clip_workspace(n, ctypes.byref(size)), L)
+    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    with _guard(dev):
+        _abi.check(L.goi_clip_gradients(
+            n, pointers(*[g.data_ptr() for g, _ in pairs]), pointers(*[o.data_ptr() for _, o in pairs]),
+            longs(*[g.numel() for g, _ in pairs]), ints(*[_TYPES[g.dtype] for g, _ in pairs]),
+            ints(*[_TYPES[o.dtype] for _, o in pairs]), max_norm, norm.data_ptr(), ws.data_ptr(), size.value, _stream(dev)), L)
+    return norm

@@ -12,7 +12,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 SRC = [HERE / "csrc" / f for f in ("goi_b2.hip", "goi_b2_rig.hip", "goi_b2_island.hip", "goi_b2_w1.hip",
                                     "goi_b2_w2.hip", "goi_b2_w4.hip", "goi_b2_w8.hip", "policy_attention.hip",
-                                    "policy_attention_dq.hip", "policy_attention_dkv.hip")]
+                                    "policy_attention_dq.hip", "policy_attention_dkv.hip", "policy_norm.hip",
+                                    "policy_int8.hip", "policy_clip.hip")]
 OUT = HERE / "lib" / "libgoi_b2.so"
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-shared", "-std=c++17", "-ffp-contract=off", "-fno-fast-math",

@@ -1,0 +1,204 @@
+// policy_clip.hip - the global norm of many gradients and their clipping (include/goi_policy.h). Two passes over the
+// tensors, a launch for up to kTensors of them each: their addresses travel in the kernel's arguments, so nothing is copied to the
+// device and nothing is kept between calls. Bound by memory.
+#include <algorithm>
+#include <climits>
+
+#include "policy.hpp"
+
+namespace goi {
+namespace {
+
+constexpr int kTensors = 112;      // tables of 32 bytes a tensor within the 4 KB of kernel arguments
+constexpr int kSegment = 16384;    // elements of a tensor that a block takes at a time
+constexpr int kBlocks = 1024;      // blocks of a launch, and partial sums it leaves: 4 a CU
+
+struct Tensors {
+    const void* grad[kTensors];
+    void* out[kTensors];
+    int64_t size[kTensors];
+    int32_t first[kTensors];   // segments before this tensor's
+    uint8_t type[kTensors], out_type[kTensors];
+    int count, segments;
+};
+
+// tensor of segment s: the last one whose first segment is not after s (empty tensors hold none)
+__device__ __forceinline__ int tensor_of(const Tensors& t, int s) {
+    int lo = 0, hi = t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (t.first[mid] <= s) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T>
+__device__ __forceinline__ double squares(const T* x, int n) {
+    constexpr int V = 16 / sizeof(T);
+    double s = 0.0;
+    if (((uintptr_t)x & 15) == 0) {
+        const int whole = n / V;
+        for (int i = threadIdx.x; i < whole; i += blockDim.x) {
+            union {
+                int4_t raw;
+                T e[V];
+            } u;
+            u.raw = reinterpret_cast<const int4_t*>(x)[i];
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += (double)(float)u.e[k] * (double)(float)u.e[k];
+        }
+        for (int i = whole * V + threadIdx.x; i < n; i += blockDim.x) s += (double)(float)x[i] * (double)(float)x[i];
+    } else {
+        for (int i = threadIdx.x; i < n; i += blockDim.x) s += (double)(float)x[i] * (double)(float)x[i];
+    }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum(double x, double* shared) {
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (shared[0] + shared[1]) + (shared[2] + shared[3]);
+}
+
+__global__ void __launch_bounds__(256) k_square_sums(const Tensors t, double* parts) {
+    __shared__ double shared[4];
+    double s = 0.0;
+    for (int seg = blockIdx.x; seg < t.segments; seg += gridDim.x) {
+        const int i = tensor_of(t, seg);
+        const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
+        const int n = (int)min((int64_t)kSegment, t.size[i] - at);
+        if (t.type[i] == GOI_F32) s += squares(static_cast<const float*>(t.grad[i]) + at, n);
+        else if (t.type[i] == GOI_F16) s += squares(static_cast<const f16*>(t.grad[i]) + at, n);
+        else s += squares(static_cast<const bf16*>(t.grad[i]) + at, n);
+    }
+    s = block_sum(s, shared);
+    if (threadIdx.x == 0) parts[blockIdx.x] = s;
+}
+
+template <typename T, typename U>
+__device__ __forceinline__ void scale(const T* x, U* y, int n, float f) {
+    constexpr int V = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
+    struct __attribute__((aligned(sizeof(T) * V))) In { T e[V]; };
+    struct __attribute__((aligned(sizeof(U) * V))) Out { U e[V]; };
+    int done = 0;
+    if ((((uintptr_t)x & (sizeof(In) - 1)) | ((uintptr_t)y & (sizeof(Out) - 1))) == 0) {
+        const int whole = n / V;
+        for (int i = threadIdx.x; i < whole; i += blockDim.x) {
+            const In a = reinterpret_cast<const In*>(x)[i];
+            Out b;
+#pragma unroll
+            for (int k = 0; k < V; ++k) b.e[k] = (U)((float)a.e[k] * f);
+            reinterpret_cast<Out*>(y)[i] = b;
+        }
+        done = whole * V;
+    }
+    for (int i = done + threadIdx.x; i < n; i += blockDim.x) y[i] = (U)((float)x[i] * f);
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_to(const T* x, void* out, int type, int64_t at, int n, float f) {
+    if (type == GOI_F32) scale(x, static_cast<float*>(out) + at, n, f);
+    else if (type == GOI_F16) scale(x, static_cast<f16*>(out) + at, n, f);
+    else scale(x, static_cast<bf16*>(out) + at, n, f);
+}
+
+// Each block sums the partial sums itself (a few KB from L2) in the same order. The segments run backwards, so that the
+// first ones read are those that the pass before read last and the last-level cache may still hold.
+__global__ void __launch_bounds__(256) k_clip(const Tensors t, const double* parts, int count, float max_norm, float* norm) {
+    __shared__ double shared[4];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < count; i += 256) s += parts[i];
+    const float total = (float)sqrt(block_sum(s, shared));
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
+    float f = max_norm / (total + 1e-6f);
+    f = f > 1.0f ? 1.0f : f;
+    for (int seg = t.segments - 1 - (int)blockIdx.x; seg >= 0; seg -= gridDim.x) {
+        const int i = tensor_of(t, seg);
+        if (t.out[i] == t.grad[i] && f == 1.0f) continue;
+        const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
+        const int n = (int)min((int64_t)kSegment, t.size[i] - at);
+        if (t.type[i] == GOI_F32) scale_to(static_cast<const float*>(t.grad[i]) + at, t.out[i], t.out_type[i], at, n, f);
+        else if (t.type[i] == GOI_F16) scale_to(static_cast<const f16*>(t.grad[i]) + at, t.out[i], t.out_type[i], at, n, f);
+        else scale_to(static_cast<const bf16*>(t.grad[i]) + at, t.out[i], t.out_type[i], at, n, f);
+    }
+}
+
+int launches(int count) { return std::max(1, (count + kTensors - 1) / kTensors); }
+
+}  // namespace
+}  // namespace goi
+
+using namespace goi;
+
+extern "C" {
+
+int32_t goi_clip_workspace(int32_t count, uint64_t* bytes) {
+    if (count < 0 || !bytes) return policy_error(GOI_E_ARG, "goi_clip_workspace: bad arguments");
+    *bytes = (uint64_t)launches(count) * kBlocks * sizeof(double);
+    return GOI_OK;
+}
+
+int32_t goi_clip_gradients(int32_t count, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* types,
+                           const int32_t* out_types, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes,
+                           void* hip_stream) {
+    const char* const who = "goi_clip_gradients";
+    if (count < 0 || !norm || (count > 0 && (!grads || !sizes || !types || (outs && !out_types))))
+        return policy_error(GOI_E_ARG, "%s: null or negative argument", who);
+    if (!(max_norm >= 0.0f)) return policy_error(GOI_E_ARG, "%s: max_norm is negative or NaN", who);
+    uint64_t bytes = 0;
+    goi_clip_workspace(count, &bytes);
+    if (!workspace || bytes > workspace_bytes || (uintptr_t)workspace & 15)
+        return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
+    const auto known = [](int type) { return type == GOI_F32 || type == GOI_F16 || type == GOI_BF16; };
+    for (int i = 0; i < count; ++i) {
+        if (sizes[i] < 0 || (sizes[i] > 0 && (!grads[i] || (outs && !outs[i]))))
+            return policy_error(GOI_E_ARG, "%s: tensor %d is null or negative", who, i);
+        if (!known(types[i]) || (outs && !known(out_types[i])))
+            return policy_error(GOI_E_UNSUPPORTED, "%s: tensor %d is of an unknown type", who, i);
+        const int size = types[i] == GOI_F32 ? 4 : 2;
+        if ((uintptr_t)grads[i] % size || (outs && (uintptr_t)outs[i] % (out_types[i] == GOI_F32 ? 4 : 2)))
+            return policy_error(GOI_E_ARG, "%s: tensor %d is misaligned", who, i);
+        if (outs && outs[i] == grads[i] && out_types[i] != types[i])
+            return policy_error(GOI_E_ARG, "%s: tensor %d in place is of another type", who, i);
+        if (sizes[i] / kSegment > INT_MAX / kTensors - 1)
+            return policy_error(GOI_E_UNSUPPORTED, "%s: tensor %d is too large", who, i);
+    }
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    double* const parts = static_cast<double*>(workspace);
+    const auto table = [&](int l, Tensors* t) {
+        t->count = std::min(kTensors, count - l * kTensors);
+        t->segments = 0;
+        for (int i = 0; i < t->count; ++i) {
+            const int j = l * kTensors + i;
+            t->grad[i] = grads[j];
+            t->out[i] = outs ? outs[j] : nullptr;
+            t->size[i] = sizes[j];
+            t->type[i] = (uint8_t)types[j];
+            t->out_type[i] = outs ? (uint8_t)out_types[j] : 0;
+            t->first[i] = t->segments;
+            t->segments += (int)((sizes[j] + kSegment - 1) / kSegment);
+        }
+        return std::min(kBlocks, std::max(1, t->segments));
+    };
+    Tensors t;
+    int n_parts = 0;
+    for (int l = 0; l < launches(count); ++l) {
+        const int blocks = table(l, &t);
+        hipLaunchKernelGGL(k_square_sums, dim3(blocks), dim3(256), 0, st, t, parts + n_parts);
+        n_parts += blocks;
+    }
+    for (int l = launches(count) - 1; l >= 0; --l) {
+        int blocks = table(l, &t);
+        if (!outs) {
+            t.segments = 0;
+            blocks = 1;
+            if (l > 0) continue;
+        }
+        hipLaunchKernelGGL(k_clip, dim3(blocks), dim3(256), 0, st, t, parts, n_parts, max_norm, l == 0 ? norm : nullptr);
+    }
+    return launch_error(who);
+}
+
+}  // extern "C"

@@ -1,0 +1,398 @@
+// policy_norm.hip - root-mean-square norm of rows with the residual's addition, in the type or in 8 bits, and its gradient
+// (include/goi_policy.h). Bound by memory: each element is read once into registers, reduced, and written once.
+//
+// A row is held by `tpr` lanes of one wave (a power of two up to 64) or, past 2048 elements, by a block of 128 .. 1024
+// threads, 32 elements a thread: the fewest lanes that hold it, so that a lane has several 16-byte loads in flight. A thread's chunks
+// of VEC elements lie tpr * VEC apart, so neighbouring lanes read neighbouring chunks. VEC is the widest of 8, 4, 2 and 1 that divides
+// the width and fits the alignment of every pointer and stride.
+#include <algorithm>
+
+#include "policy.hpp"
+
+namespace goi {
+namespace {
+
+constexpr int kPer = 32;  // elements a thread
+
+template <typename T, int VEC>
+struct __attribute__((aligned(sizeof(T) * VEC))) Chunk {
+    T e[VEC];
+};
+
+template <int TPR_WAVES>
+__device__ __forceinline__ float row_sum(float x, int tpr, float* shared) {
+    for (int d = min(tpr, 64) / 2; d; d >>= 1) x += __shfl_xor(x, d);
+    if constexpr (TPR_WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = 0.0f;
+        for (int w = 0; w < (int)blockDim.x / 64; ++w) x += shared[w];
+    }
+    return x;
+}
+
+// the larger, and NaN if either is
+__device__ __forceinline__ float max_or_nan(float a, float b) { return a > b || a != a ? a : b; }
+
+template <int TPR_WAVES>
+__device__ __forceinline__ float row_max(float x, int tpr, float* shared) {
+    for (int d = min(tpr, 64) / 2; d; d >>= 1) x = max_or_nan(x, __shfl_xor(x, d));
+    if constexpr (TPR_WAVES > 1) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = shared[0];
+        for (int w = 1; w < (int)blockDim.x / 64; ++w) x = max_or_nan(x, shared[w]);
+    }
+    return x;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const T* p, float* f) {
+    const Chunk<T, VEC> c = *reinterpret_cast<const Chunk<T, VEC>*>(p);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = (float)c.e[e];
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, const float* f) {
+    Chunk<T, VEC> c;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) c.e[e] = (T)f[e];
+    *reinterpret_cast<Chunk<T, VEC>*>(p) = c;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void load_weight(const void* w, int type, int col, float* f) {
+    if (type != GOI_F32) return load<T, VEC>(static_cast<const T*>(w) + col, f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = static_cast<const float*>(w)[col + e];
+}
+
+template <typename T, int VEC, int TPR_WAVES, bool kInt8>
+__global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_norm(const GoiNorm a, int tpr) {
+    __shared__ float shared[16];
+    constexpr int N = kPer / VEC;
+    const int row = TPR_WAVES > 1 ? blockIdx.x : blockIdx.x * (256 / tpr) + threadIdx.x / tpr, sub = threadIdx.x % tpr;
+    const bool live = row < a.rows;  // lanes without a row stay for the exchanges
+    const int64_t at = live ? row : 0;
+    const T* const x = static_cast<const T*>(a.x) + at * a.x_stride;
+    const T* const res = a.residual ? static_cast<const T*>(a.residual) + at * a.residual_stride : nullptr;
+    float f[kPer];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int col = (j * tpr + sub) * VEC;
+        float* const c = f + j * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) c[e] = 0.0f;
+        if (col < a.width) {
+            load<T, VEC>(x + col, c);
+            if (res) {
+                float y[VEC];
+                load<T, VEC>(res + col, y);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) c[e] = (float)(T)(c[e] + y[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum += c[e] * c[e];
+    }
+    sum = row_sum<TPR_WAVES>(sum, tpr, shared);
+    const float inv = 1.0f / sqrtf(sum / (float)a.width + a.eps);
+    if (live && sub == 0 && a.inv) a.inv[row] = inv;
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int col = (j * tpr + sub) * VEC;
+        if (col >= a.width) continue;
+        float* const c = f + j * VEC;
+        if (res && live) store<T, VEC>(static_cast<T*>(a.r) + at * a.r_stride + col, c);
+        float w[VEC];
+        load_weight<T, VEC>(a.weight, a.weight_type, col, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) c[e] = c[e] * inv * w[e];
+        if constexpr (kInt8) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = max_or_nan(top, fabsf(c[e]));
+        } else if (live) {
+            store<T, VEC>(static_cast<T*>(a.y) + at * a.y_stride + col, c);
+        }
+    }
+    if constexpr (kInt8) {
+        top = row_max<TPR_WAVES>(top, tpr, shared);
+        const bool finite = top <= 3.4028235e38f;  // neither NaN nor infinity
+        const float scale = !finite ? NAN : top > 0.0f ? top / 127.0f : 1.0f;
+        if (live && sub == 0) a.scales[row] = scale;
+        if (top < 1e-30f) {  // the inverse of the scale would overflow or lose bits
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) f[x] /= scale;
+        } else {
+            const float back = 127.0f / top;
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) f[x] *= back;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col >= a.width || !live) continue;
+            Chunk<int8_t, VEC> c;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                c.e[e] = finite ? (int8_t)fminf(fmaxf(rintf(f[j * VEC + e]), -127.0f), 127.0f) : 0;
+            *reinterpret_cast<Chunk<int8_t, VEC>*>(a.values + at * a.values_stride + col) = c;
+        }
+    }
+}
+
+// dx row by row; dweight's sums stay in the thread's registers over the block's rows (a thread keeps its columns), then one
+// part a block.
+template <typename T, int VEC, int TPR_WAVES>
+__global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_norm_backward(const GoiNormBackward a, int tpr,
+                                                                                            float* parts) {
+    __shared__ float shared[16];
+    extern __shared__ float columns[];  // [width], where several rows share a block
+    constexpr int N = kPer / VEC;
+    const int per = TPR_WAVES > 1 ? 1 : 256 / tpr, group = TPR_WAVES > 1 ? 0 : threadIdx.x / tpr, sub = threadIdx.x % tpr;
+    float w[kPer], dw[kPer];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int col = (j * tpr + sub) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[j * VEC + e] = dw[j * VEC + e] = 0.0f;
+        if (col < a.width) load_weight<T, VEC>(a.weight, a.weight_type, col, w + j * VEC);
+    }
+    for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += (int64_t)gridDim.x * per) {
+        const bool live = base + group < a.rows;
+        const int64_t row = live ? base + group : 0;
+        const T* const dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
+        const T* const r = static_cast<const T*>(a.r) + row * a.r_stride;
+        const float inv = a.inv[row];
+        float g[kPer], x[kPer];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            float* const gc = g + j * VEC;
+            float* const xc = x + j * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) gc[e] = xc[e] = 0.0f;
+            if (col < a.width && live) {
+                load<T, VEC>(dy + col, gc);
+                load<T, VEC>(r + col, xc);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                dw[j * VEC + e] += gc[e] * xc[e] * (live ? inv : 0.0f);
+                gc[e] *= w[j * VEC + e];
+                sum += gc[e] * xc[e];
+            }
+        }
+        sum = row_sum<TPR_WAVES>(sum, tpr, shared);
+        const float along = sum / (float)a.width * inv * inv;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col >= a.width || !live) continue;
+            float y[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] = 0.0f;
+            if (a.dresidual) load<T, VEC>(static_cast<const T*>(a.dresidual) + row * a.dresidual_stride + col, y);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] += inv * (g[j * VEC + e] - x[j * VEC + e] * along);
+            store<T, VEC>(static_cast<T*>(a.dx) + row * a.dx_stride + col, y);
+        }
+    }
+    float* const part = parts + (int64_t)blockIdx.x * a.width;
+    if (per == 1) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col >= a.width) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[col + e] = dw[j * VEC + e];
+        }
+        return;
+    }
+    // the block's rows one after another, in a fixed order
+    for (int x = threadIdx.x; x < a.width; x += blockDim.x) columns[x] = 0.0f;
+    for (int k = 0; k < per; ++k) {
+        __syncthreads();
+        if (group != k) continue;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col >= a.width) continue;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) columns[col + e] += dw[j * VEC + e];
+        }
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < a.width; x += blockDim.x) part[x] = columns[x];
+}
+
+// dweight from the blocks' parts
+__global__ void __launch_bounds__(256) k_column_sum(const float* parts, int count, int width, void* out, int type) {
+    __shared__ float part[16][17];
+    const int sub = threadIdx.x >> 4, col = blockIdx.x * 16 + (threadIdx.x & 15);
+    float s = 0.0f;
+    if (col < width)
+        for (int r = sub; r < count; r += 16) s += parts[(int64_t)r * width + col];
+    part[sub][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (sub || col >= width) return;
+    s = 0.0f;
+    for (int r = 0; r < 16; ++r) s += part[r][threadIdx.x];
+    if (type == GOI_F32) static_cast<float*>(out)[col] = s;
+    else if (type == GOI_F16) static_cast<f16*>(out)[col] = (f16)s;
+    else static_cast<bf16*>(out)[col] = (bf16)s;
+}
+
+// ---------------------------------------------------------------- host
+
+constexpr int kMaxWidth = 1024 * kPer;
+constexpr int kParts = 1024;  // blocks of the backward pass: 4 a CU
+
+int lanes_for(int width) {
+    int tpr = 8;
+    while (tpr < 1024 && tpr * kPer < width) tpr *= 2;
+    return tpr;
+}
+
+// Narrows vec to what p and its row stride (elements of `size` bytes) allow
+void narrow(int* vec, const void* p, int64_t stride, int size) {
+    if (!p) return;
+    while (*vec > 1 && (((uintptr_t)p | (uintptr_t)(stride * size)) & (uintptr_t)(*vec * size - 1))) *vec /= 2;
+}
+
+int element_size(int type) { return type == GOI_F32 ? 4 : 2; }
+
+int check(int rows, int width, int type, int weight_type, const char* who) {
+    if (rows < 0 || width < 1) return policy_error(GOI_E_ARG, "%s: negative rows or no width", who);
+    if (type != GOI_F32 && type != GOI_F16 && type != GOI_BF16) return policy_error(GOI_E_UNSUPPORTED, "%s: unknown type", who);
+    if (weight_type != type && weight_type != GOI_F32)
+        return policy_error(GOI_E_UNSUPPORTED, "%s: the weight is of another 16-bit type", who);
+    if (width > kMaxWidth) return policy_error(GOI_E_UNSUPPORTED, "%s: width above %d", who, kMaxWidth);
+    return GOI_OK;
+}
+
+template <typename T, int VEC, bool kInt8>
+void launch_norm(const GoiNorm& a, int tpr, hipStream_t st) {
+    if (tpr <= 64)
+        hipLaunchKernelGGL((k_rms_norm<T, VEC, 1, kInt8>), dim3((a.rows + 256 / tpr - 1) / (256 / tpr)), dim3(256), 0, st, a, tpr);
+    else
+        hipLaunchKernelGGL((k_rms_norm<T, VEC, 16, kInt8>), dim3(a.rows), dim3(tpr), 0, st, a, tpr);
+}
+template <typename T, int VEC>
+void launch_norm(const GoiNorm& a, int tpr, hipStream_t st) {
+    if (a.values) launch_norm<T, VEC, true>(a, tpr, st);
+    else launch_norm<T, VEC, false>(a, tpr, st);
+}
+template <typename T>
+void launch_norm(const GoiNorm& a, int vec, int tpr, hipStream_t st) {
+    if (vec == 8) {
+        if constexpr (sizeof(T) == 2) launch_norm<T, 8>(a, tpr, st);
+    } else if (vec == 4) launch_norm<T, 4>(a, tpr, st);
+    else if (vec == 2) launch_norm<T, 2>(a, tpr, st);
+    else launch_norm<T, 1>(a, tpr, st);
+}
+
+template <typename T, int VEC>
+void launch_backward(const GoiNormBackward& a, int tpr, int blocks, float* parts, hipStream_t st) {
+    if (tpr <= 64)
+        hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 1>), dim3(blocks), dim3(256), a.width * sizeof(float), st, a, tpr, parts);
+    else
+        hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 16>), dim3(blocks), dim3(tpr), 0, st, a, tpr, parts);
+}
+template <typename T>
+void launch_backward(const GoiNormBackward& a, int vec, int tpr, int blocks, float* parts, hipStream_t st) {
+    if (vec == 8) {
+        if constexpr (sizeof(T) == 2) launch_backward<T, 8>(a, tpr, blocks, parts, st);
+    } else if (vec == 4) launch_backward<T, 4>(a, tpr, blocks, parts, st);
+    else if (vec == 2) launch_backward<T, 2>(a, tpr, blocks, parts, st);
+    else launch_backward<T, 1>(a, tpr, blocks, parts, st);
+}
+
+int backward_blocks(int rows, int width) {
+    const int tpr = lanes_for(width), per = tpr <= 64 ? 256 / tpr : 1;
+    return (int)std::min<int64_t>(kParts, ((int64_t)rows + per - 1) / per);
+}
+
+int widest(int width, int type) {
+    int vec = type == GOI_F32 ? 4 : 8;
+    while (width % vec) vec /= 2;
+    return vec;
+}
+
+}  // namespace
+}  // namespace goi
+
+using namespace goi;
+
+extern "C" {
+
+int32_t goi_rms_norm(const GoiNorm* a, void* hip_stream) {
+    const char* const who = "goi_rms_norm";
+    if (!a) return policy_error(GOI_E_ARG, "%s: null argument", who);
+    const int rc = check(a->rows, a->width, a->type, a->weight_type, who);
+    if (rc != GOI_OK) return rc;
+    if (a->rows == 0) return GOI_OK;
+    if (!a->values == !a->y) return policy_error(GOI_E_ARG, "%s: one of y and values", who);
+    if (!a->x || !a->weight || (a->residual && !a->r) || (a->values && !a->scales))
+        return policy_error(GOI_E_ARG, "%s: null argument", who);
+    const int size = element_size(a->type);
+    int vec = widest(a->width, a->type);
+    narrow(&vec, a->x, a->x_stride, size);
+    narrow(&vec, a->residual, a->residual_stride, size);
+    narrow(&vec, a->r, a->residual ? a->r_stride : 0, size);
+    narrow(&vec, a->y, a->y ? a->y_stride : 0, size);
+    narrow(&vec, a->weight, 0, size);
+    narrow(&vec, a->values, a->values_stride, 1);
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    const int tpr = lanes_for(a->width);
+    if (a->type == GOI_F32) launch_norm<float>(*a, vec, tpr, st);
+    else if (a->type == GOI_F16) launch_norm<f16>(*a, vec, tpr, st);
+    else launch_norm<bf16>(*a, vec, tpr, st);
+    return launch_error(who);
+}
+
+int32_t goi_rms_norm_backward_workspace(int32_t rows, int32_t width, uint64_t* bytes) {
+    const char* const who = "goi_rms_norm_backward_workspace";
+    if (!bytes) return policy_error(GOI_E_ARG, "%s: null argument", who);
+    const int rc = check(rows, width, GOI_F32, GOI_F32, who);
+    if (rc != GOI_OK) return rc;
+    *bytes = (uint64_t)backward_blocks(rows, width) * width * sizeof(float);
+    return GOI_OK;
+}
+
+int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_t workspace_bytes, void* hip_stream) {
+    const char* const who = "goi_rms_norm_backward";
+    if (!a) return policy_error(GOI_E_ARG, "%s: null argument", who);
+    const int rc = check(a->rows, a->width, a->type, a->weight_type, who);
+    if (rc != GOI_OK) return rc;
+    if (!a->dweight || !a->weight || (a->rows > 0 && (!a->dy || !a->r || !a->inv || !a->dx)))
+        return policy_error(GOI_E_ARG, "%s: null argument", who);
+    const int blocks = backward_blocks(a->rows, a->width);
+    const uint64_t bytes = (uint64_t)blocks * a->width * sizeof(float);
+    if (bytes > workspace_bytes || (bytes && (!workspace || (uintptr_t)workspace & 15)))
+        return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
+    const hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    float* const parts = static_cast<float*>(workspace);
+    if (a->rows > 0) {
+        const int size = element_size(a->type);
+        int vec = widest(a->width, a->type);
+        narrow(&vec, a->dy, a->dy_stride, size);
+        narrow(&vec, a->r, a->r_stride, size);
+        narrow(&vec, a->dresidual, a->dresidual_stride, size);
+        narrow(&vec, a->dx, a->dx_stride, size);
+        narrow(&vec, a->weight, 0, size);
+        const int tpr = lanes_for(a->width);
+        if (a->type == GOI_F32) launch_backward<float>(*a, vec, tpr, blocks, parts, st);
+        else if (a->type == GOI_F16) launch_backward<f16>(*a, vec, tpr, blocks, parts, st);
+        else launch_backward<bf16>(*a, vec, tpr, blocks, parts, st);
+    }
+    hipLaunchKernelGGL(k_column_sum, dim3((a->width + 15) / 16), dim3(256), 0, st, parts, blocks, a->width, a->dweight,
+                       a->weight_type);
+    return launch_error(who);
+}
+
+}  // extern "C"

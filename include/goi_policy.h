@@ -77,6 +77,81 @@ int32_t goi_attention_forward(const GoiAttention* a, void* workspace, uint64_t w
 /* The gradients of q, k, v and bias from dout, out and stats; the probabilities are computed again from q, k and stats. */
 int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t workspace_bytes, void* hip_stream);
 
+/* Root-mean-square norm of rows with the residual's addition. x, residual, r, y: [rows, width] of `type` with row strides in elements,
+ * the last axis contiguous; weight [width] of weight_type (type or GOI_F32).
+ *   r = round(x + residual)           (the residual stream is held in its type; without a residual r is x and not written)
+ *   inv = 1 / sqrt(mean(r^2) + eps),  y = round(r * inv * weight)
+ * inv [rows] float32 may be null. Sums are float32. width 1 .. 32768. */
+typedef struct GoiNorm {
+    int32_t rows, width, type, weight_type;
+    float eps;
+    const void* x;
+    int64_t x_stride;
+    const void* residual; /* or null */
+    int64_t residual_stride;
+    const void* weight;
+    void* r; /* required with a residual */
+    int64_t r_stride;
+    void* y; /* y or values */
+    int64_t y_stride;
+    /* In 8 bits instead of y: scale = max|r * inv * weight| / 127 (1 for a row of zeros), values = the nearest whole number
+     * of r * inv * weight / scale. A row with a value that is not finite has a scale of NaN. */
+    int8_t* values;
+    int64_t values_stride;
+    float* scales; /* [rows] */
+    float* inv;    /* [rows] */
+} GoiNorm;
+int32_t goi_rms_norm(const GoiNorm* a, void* hip_stream);
+
+/* Its gradient from dy, r, inv and, if the residual stream's own gradient comes back from later layers, dresidual:
+ *   g = dy * weight,  dx = inv * (g - r * inv^2 * mean(g * r)) + dresidual   (the gradient of x and of residual alike)
+ *   dweight = sum over rows of dy * r * inv   (float32, in a fixed order; of weight_type) */
+typedef struct GoiNormBackward {
+    int32_t rows, width, type, weight_type;
+    const void* dy;
+    int64_t dy_stride;
+    const void* r;
+    int64_t r_stride;
+    const void* dresidual; /* or null */
+    int64_t dresidual_stride;
+    const void* weight;
+    const float* inv;
+    void* dx;
+    int64_t dx_stride;
+    void* dweight;
+} GoiNormBackward;
+int32_t goi_rms_norm_backward_workspace(int32_t rows, int32_t width, uint64_t* bytes);
+int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_t workspace_bytes, void* hip_stream);
+
+/* Product in 8-bit integers with a scale for each row (token) and each channel:
+ *   y[m, n] = round( x_scales[m] * w_scales[n] * sum_k x[m, k] w[n, k]  +  bias[n] )
+ * x [rows, width] and w [channels, width] int8, 16-byte aligned with row strides that are multiples of 16 bytes (what lies
+ * between width and the stride is not read); y [rows, channels] of `type`
+ * (any of the three) with a row stride in elements. The sum is exact: int32, so width <= 131071. */
+typedef struct GoiInt8 {
+    int32_t rows, channels, width, type, bias_type; /* bias_type: type or GOI_F32 */
+    const int8_t* x;
+    int64_t x_stride;
+    const float* x_scales;
+    const int8_t* w;
+    int64_t w_stride;
+    const float* w_scales;
+    const void* bias; /* [channels], or null */
+    void* y;
+    int64_t y_stride;
+} GoiInt8;
+int32_t goi_linear_int8(const GoiInt8* a, void* hip_stream);
+
+/* The global norm of `count` tensors and their clipping: norm = sqrt(sum of squares over all of them) (sums in float64, so no
+ * value that a type holds overflows), factor = min(1, max_norm / (norm + 1e-6)), outs[i] = round(grads[i] * factor). A norm of
+ * infinity or NaN gives the factor that this formula gives (0 or NaN). grads[i] is contiguous, sizes[i] elements of types[i]; outs[i]
+ * of out_types[i] may be grads[i] itself (it is then left alone where factor is 1) and no other overlap is allowed. The
+ * arrays are host memory, read before the call returns. norm: one float32 on the device. outs may be null: the norm only. */
+int32_t goi_clip_workspace(int32_t count, uint64_t* bytes);
+int32_t goi_clip_gradients(int32_t count, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* types,
+                           const int32_t* out_types, float max_norm, float* norm, void* workspace, uint64_t workspace_bytes,
+                           void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
