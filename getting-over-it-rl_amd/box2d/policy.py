@@ -51,7 +51,8 @@ def _stream(dev):
 
 def _rows(x):
     """x (worlds, steps, heads, dim) as the attention kernels read it, and its strides of worlds, steps and heads."""
-    if x.data_ptr() % 16 or x.stride(3) != 1 or any(x.stride(d) % 8 and x.shape[d] > 1 for d in range(3)):
+    if (x.data_ptr() % 16 or x.stride(3) != 1 or any(x.stride(d) % 8 and x.shape[d] > 1 for d in range(3))
+            or any(x.stride(d) >= 1 << 24 and x.shape[d] > 1 for d in (1, 2))):
         x = x.clone(memory_format=torch.contiguous_format)
     s = x.stride()
     return x, _abi._I64x3(*(s[d] if x.shape[d] > 1 else 0 for d in range(3)))

@@ -63,17 +63,36 @@ __device__ __forceinline__ int mfma_row(int r, int half) { return (r & 3) + 8 * 
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// the value of the lane 32 away
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// the values of a lane and of the lane 32 away, in the same order in both
+__device__ __forceinline__ float2 both_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_max(float x) {
+    const float2 y = both_halves(x);
+    return fmaxf(y.x, y.y);
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const float2 y = both_halves(x);
+    return y.x + y.y;
+}
 
+// The smallest and the largest of the wave's values: within rows of 16 lanes (shifts by 1, 2, 4, 8), then row to row (the
+// last lane of a row, then of two); lane 63 has the result.
+template <int kShift>
+__device__ __forceinline__ int shifted(int x) {
+    return __builtin_amdgcn_update_dpp(x, x, kShift, 0xf, 0xf, false);
+}
 __device__ __forceinline__ int wave_min(int x) {
-    for (int d = 32; d; d >>= 1) x = min(x, __shfl_xor(x, d));
-    return __builtin_amdgcn_readfirstlane(x);
+    x = min(x, shifted<0x111>(x));
+    x = min(x, shifted<0x112>(x));
+    x = min(x, shifted<0x114>(x));
+    x = min(x, shifted<0x118>(x));
+    x = min(x, shifted<0x142>(x));
+    x = min(x, shifted<0x143>(x));
+    return __builtin_amdgcn_readlane(x, 63);
 }
-__device__ __forceinline__ int wave_max(int x) {
-    for (int d = 32; d; d >>= 1) x = max(x, __shfl_xor(x, d));
-    return __builtin_amdgcn_readfirstlane(x);
-}
+__device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
 
 // Block b's place in a grid of nb blocks so that each of the 8 XCDs (block b runs on XCD b % 8, each with its own L2) takes
 // one contiguous range of places: a bijection for any nb.

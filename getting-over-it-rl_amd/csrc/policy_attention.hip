@@ -7,158 +7,201 @@
 namespace goi {
 namespace {
 
+// The outputs of a wave's 32 rows pair by pair, from their maxima and sums
+template <typename T, bool kSplit>
+__device__ void careful_rows(const AttnRun& A, int n, int g, int L, int split, int m0, const float* table, const Row& mine,
+                             float my_top, float my_sum, int lane) {
+    for (int r = 0; r < 32 && m0 + r < A.rows; ++r) {
+        const int i = step_of(A, m0 + r), hl = m0 + r - i * A.group, head = g * A.group + hl;
+        const int lo = __shfl(mine.lo, r), hi = __shfl(mine.hi, r);
+        const float top = __shfl(my_top, r), sum = __shfl(my_sum, r);
+        const float2 q = two_elements(A.q.at<T>(n, i, head), A.dim, lane);
+        const float* const bias = A.bias ? table + hl * A.table + kPad : nullptr;
+        float2 o = make_float2(0.0f, 0.0f);
+        for (int key = lo; key < hi; ++key) {
+            const float2 k = two_elements(A.k.at<T>(n, key, g), A.dim, lane), v = two_elements(A.v.at<T>(n, key, g), A.dim, lane);
+            const float s = careful_score(A, q, k, bias, L - A.q_steps + i - key);
+            const float p = exp2_fast(s - (top == -INFINITY ? 0.0f : top));
+            o.x += p * v.x;
+            o.y += p * v.y;
+        }
+        if (kSplit) {
+            float* const to = A.part_o + (((int64_t)split * A.n_worlds * A.kv_heads + n * A.kv_heads + g) * A.rows + m0 + r) * A.dim;
+            if (lane < A.dim) to[lane] = o.x;
+            if (lane + 64 < A.dim) to[lane + 64] = o.y;
+        } else {
+            T* const to = A.out.at<T>(n, i, head);
+            const float f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            if (lane < A.dim) to[lane] = (T)(o.x * f);
+            if (lane + 64 < A.dim) to[lane + 64] = (T)(o.y * f);
+        }
+    }
+}
+
 // NW waves of 32 packed rows each share tiles of KT keys. Two tiles of LDS (one for a single wave, which needs no barrier):
 // the next tile's loads are in flight while this one is computed.
 template <typename T, int DP, int NW, bool kSplit>
-__global__ void __launch_bounds__(64 * NW) k_attention(const AttnRun A) {
-    constexpr int NT = 64 * NW, KT = NW == 1 && DP == 128 ? 32 : 64, KB = KT / 32, NBUF = NW == 1 ? 1 : 2;
+__global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_attention(const AttnRun A) {
+    constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int range[2][NW];
     T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][keys, values][KT][DP]
     float* const table = reinterpret_cast<float*>(lds + NBUF * 2 * KT * DP * sizeof(T));
-    const GoiAttention& a = A.a;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
-    int place = xcd_place(blockIdx.x, gridDim.x);
-    // the later row tiles of a causal window see the most keys: they go first
-    const int tile = A.tiles - 1 - place % A.tiles;
-    place /= A.tiles;
-    const int split = kSplit ? place % A.splits : 0;
-    if (kSplit) place /= A.splits;
-    const int n = place / a.kv_heads, g = place - n * a.kv_heads;
-
-    const int L = history(A, n), m = (tile * NW + wave) * 32 + (lane & 31);
-    Row row = make_row(A, n, L, m);
-    if (kSplit) {
-        row.lo = max(row.lo, split * A.span);
-        row.hi = min(row.hi, (split + 1) * A.span);
-        if (row.hi <= row.lo) row.lo = row.hi = 0;
-    }
-    const BlockInfo blk = make_block(row);
-    if (lane == 0) {
-        range[0][wave] = blk.lo;
-        range[1][wave] = blk.hi;
-    }
-    const float* bias = nullptr;
-    if (a.bias) {
-        stage_bias(A, g, table, tid, NT);
-        bias = table + row.hl * a.n_distances;
-    }
-    const int head = g * A.group + row.hl;
-    half8<T> q[DP / 16];
-    load_operand<T, DP>(q, static_cast<const T*>(a.q) + n * a.q_strides[0] + row.i * a.q_strides[1] + head * a.q_strides[2],
-                        row.valid, a.dim, lane);
-    __syncthreads();
-    int lo = INT_MAX, hi = 0;  // the keys that some row of the block sees
-    for (int w = 0; w < NW; ++w) {
-        lo = min(lo, range[0][w]);
-        hi = max(hi, range[1][w]);
-    }
-
-    float16_t o[DP / 32];
-    clear(o);
-    float top = -INFINITY, sum = 0.0f;
-    if (lo < hi) {
-        const T* const kp = static_cast<const T*>(a.k) + n * a.k_strides[0] + g * a.k_strides[2];
-        const T* const vp = static_cast<const T*>(a.v) + n * a.v_strides[0] + g * a.v_strides[2];
-        KeyStage<T, DP, KT, NT> ks, vs;
-        ks.load(kp, a.k_strides[1], lo, lo, hi, a.dim, tid);
-        vs.load(vp, a.v_strides[1], lo, lo, hi, a.dim, tid);
-        ks.store(tiles, lo, lo, hi, a.dim, tid);
-        vs.store(tiles + KT * DP, lo, lo, hi, a.dim, tid);
+    const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
+    if (A.bias) stage_bias(A, g, table, tid, NT);
+    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
+    for (int item = (int)((int64_t)block * A.items / A.per_head); item < end; ++item) {
+        // the later row tiles of a causal window see the most keys: they go first
+        int n = item / A.tiles, split = 0;
+        const int tile = A.tiles - 1 - (item - n * A.tiles);
+        if (kSplit) {
+            const int x = n / A.splits;
+            split = n - x * A.splits;
+            n = x;
+        }
+        const int L = history(A, n), m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
+        Row row = make_row(A, n, L, m);
+        if (kSplit) {
+            row.lo = max(row.lo, split * A.span);
+            row.hi = min(row.hi, (split + 1) * A.span);
+            if (row.hi <= row.lo) row.lo = row.hi = 0;
+        }
+        BlockInfo blk = make_block(A, L, m0, row);
+        if (kSplit) {
+            blk.lo = max(blk.lo, split * A.span);
+            blk.full_lo = max(blk.full_lo, split * A.span);
+            blk.hi = min(blk.hi, (split + 1) * A.span);
+            blk.full_hi = min(blk.full_hi, (split + 1) * A.span);
+        }
+        row.pos = min(max(row.pos, blk.pos_lo), blk.pos_hi);  // also where there is no row
+        if (NW > 1 && lane == 0) {
+            range[0][wave] = blk.lo;
+            range[1][wave] = blk.hi;
+        }
+        const float* const bias = A.bias ? table + row.hl * A.table + kPad : nullptr;
+        const int head = g * A.group + row.hl;
+        half8<T> q[DP / 16];
+        load_operand<T, DP>(q, A.q.at<T>(n, row.i, head), row.valid, A.dim, lane);
         __syncthreads();
-        int buf = 0;
-        for (int k0 = lo; k0 < hi; k0 += KT) {
-            const bool more = k0 + KT < hi;
-            if (more) {
-                ks.load(kp, a.k_strides[1], k0 + KT, lo, hi, a.dim, tid);
-                vs.load(vp, a.v_strides[1], k0 + KT, lo, hi, a.dim, tid);
+        int lo = blk.lo, hi = blk.hi;  // the keys that some row of the block sees
+        if constexpr (NW > 1) {
+            lo = INT_MAX;
+            hi = 0;
+            for (int w = 0; w < NW; ++w) {
+                lo = min(lo, range[0][w]);
+                hi = max(hi, range[1][w]);
             }
-            const T* const kt = tiles + buf * 2 * KT * DP;
-            const T* const vt = kt + KT * DP;
-            if (k0 < blk.hi && k0 + KT > blk.lo) {
-                float16_t s[KB];
-                float best = -INFINITY;
+            lo = __builtin_amdgcn_readfirstlane(lo);
+            hi = __builtin_amdgcn_readfirstlane(hi);
+        }
+
+        float16_t o[DP / 32];
+        clear(o);
+        float top = -INFINITY, sum = 0.0f;
+        bool careful = false;
+        if (lo < hi) {
+            KeyStage<T, DP, KT, NT> ks(A.k, n, g, A.dim, tid), vs(A.v, n, g, A.dim, tid);
+            ks.load(lo, hi, tid);
+            vs.load(lo, hi, tid);
+            ks.store(tiles, lo, hi, tid);
+            vs.store(tiles + KT * DP, lo, hi, tid);
+            __syncthreads();
+            int buf = 0;
+            for (int k0 = lo; k0 < hi; k0 += KT) {
+                const bool more = k0 + KT < hi;
+                if (more) {
+                    ks.load(k0 + KT, hi, tid);
+                    vs.load(k0 + KT, hi, tid);
+                }
+                const T* const kt = tiles + buf * 2 * KT * DP;
+                const T* const vt = kt + KT * DP;
+                if (k0 < blk.hi && k0 + KT > blk.lo) {
+                    float16_t s[KB];
+                    float best = -INFINITY;
 #pragma unroll
-                for (int b = 0; b < KB; ++b) {
-                    const int key0 = k0 + 32 * b;
-                    s[b] = raw_scores<T, DP>(kt, 32 * b, q, lane);
-                    scale_scores(s[b], A.c, bias, a.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
-                    if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
+                    for (int b = 0; b < KB; ++b) {
+                        const int key0 = k0 + 32 * b;
+                        s[b] = raw_scores<T, DP>(kt, 32 * b, q, lane);
+                        scale_scores(s[b], A.c, bias, A.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
+                        if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const int key = key0 + mfma_row(r, half);
+                                s[b][r] = key >= row.lo && key < row.hi ? s[b][r] : -INFINITY;
+                            }
+                            careful = careful || !finite_rows<T, DP>(vt, 32 * b, lane);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
+                    }
+                    best = half_max(best);
+                    if (__any(best > top)) {
+                        const float next = fmaxf(top, best);
+                        const float f = next == -INFINITY ? 1.0f : exp2_fast(top - next);
+                        top = next;
+                        sum *= f;
+#pragma unroll
+                        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) o[b][r] *= f;
+                    }
+                    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                    for (int b = 0; b < KB; ++b) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int key = key0 + mfma_row(r, half);
-                            s[b][r] = key >= row.lo && key < row.hi ? s[b][r] : -INFINITY;
+                            s[b][r] = exp2_fast(s[b][r] - base);
+                            sum += s[b][r];
+                        }
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const half8<T> p = to_operand<T>(s[b], x);
+#pragma unroll
+                            for (int d = 0; d < DP / 32; ++d)
+                                o[d] = mfma(column_fragment<T, DP>(vt, 32 * b + 16 * x, 32 * d, lane), p, o[d]);
                         }
                     }
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
                 }
-                best = fmaxf(best, other_half(best));
-                if (__any(best > top)) {
-                    const float next = fmaxf(top, best);
-                    const float f = next == -INFINITY ? 1.0f : exp2_fast(top - next);
-                    top = next;
-                    sum *= f;
-#pragma unroll
-                    for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[b][r] *= f;
+                if (NBUF == 1) __syncthreads();
+                else buf ^= 1;
+                if (more) {
+                    ks.store(tiles + buf * 2 * KT * DP, k0 + KT, hi, tid);
+                    vs.store(tiles + buf * 2 * KT * DP + KT * DP, k0 + KT, hi, tid);
                 }
-                const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-                for (int b = 0; b < KB; ++b) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        s[b][r] = exp2_fast(s[b][r] - base);
-                        sum += s[b][r];
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const half8<T> p = to_operand<T>(s[b], x);
-#pragma unroll
-                        for (int d = 0; d < DP / 32; ++d)
-                            o[d] = mfma(column_fragment<T, DP>(vt, 32 * b + 16 * x, 32 * d, lane), p, o[d]);
-                    }
-                }
+                __syncthreads();
             }
-            if (NBUF == 1) __syncthreads();
-            else buf ^= 1;
-            if (more) {
-                ks.store(tiles + buf * 2 * KT * DP, k0 + KT, lo, hi, a.dim, tid);
-                vs.store(tiles + buf * 2 * KT * DP + KT * DP, k0 + KT, lo, hi, a.dim, tid);
-            }
-            __syncthreads();
         }
-    }
-    sum += other_half(sum);
-    if (!row.valid) return;
-    if (kSplit) {
-        const int64_t at = ((int64_t)split * a.n_worlds * a.kv_heads + n * a.kv_heads + g) * A.rows + m;
-        if (half == 0) A.part_ml[at] = make_float2(top, sum);
-        float* const to = A.part_o + at * a.dim;
+        sum = half_sum(sum);
+        if (kSplit) {
+            if (row.valid) {
+                const int64_t at = ((int64_t)split * A.n_worlds * A.kv_heads + n * A.kv_heads + g) * A.rows + m;
+                if (half == 0) A.part_ml[at] = make_float2(top, sum);
+                float* const to = A.part_o + at * A.dim;
 #pragma unroll
-        for (int b = 0; b < DP / 32; ++b)
+                for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int d = 32 * b + 8 * x + 4 * half;
-                if (d < a.dim)
-                    *reinterpret_cast<float4_t*>(to + d) =
-                        float4_t{o[b][4 * x], o[b][4 * x + 1], o[b][4 * x + 2], o[b][4 * x + 3]};
+                    for (int x = 0; x < 4; ++x) {
+                        const int d = 32 * b + 8 * x + 4 * half;
+                        if (d < A.dim)
+                            *reinterpret_cast<float4_t*>(to + d) =
+                                float4_t{o[b][4 * x], o[b][4 * x + 1], o[b][4 * x + 2], o[b][4 * x + 3]};
+                    }
             }
-        return;
+        } else if (row.valid) {
+            store_row<T, DP>(A.out.at<T>(n, row.i, head), o, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, A.dim, half);
+            if (A.stats && half == 0) A.stats[((int64_t)n * A.heads + head) * A.q_steps + row.i] = make_float2(top, sum);
+        }
+        if (careful) careful_rows<T, kSplit>(A, n, g, L, split, m0, table, row, top, sum, lane);
+        __syncthreads();  // the next item overwrites what this one read
     }
-    T* const to = static_cast<T*>(a.out) + n * a.out_strides[0] + row.i * a.out_strides[1] + head * a.out_strides[2];
-    store_row<T, DP>(to, o, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, a.dim, half);
-    if (a.stats && half == 0)
-        reinterpret_cast<float2*>(a.stats)[((int64_t)n * a.heads + head) * a.q_steps + row.i] = make_float2(top, sum);
 }
 
 // Joins the splits of each row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, M the largest m_s. A wave a row.
 template <typename T>
 __global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
-    const GoiAttention& a = A.a;
-    const int64_t rows = (int64_t)a.n_worlds * a.kv_heads * A.rows;
+    const int64_t rows = (int64_t)A.n_worlds * A.kv_heads * A.rows;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (row >= rows) return;
@@ -167,31 +210,30 @@ __global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, x = 0.0f, y = 0.0f;
-    const bool in = 2 * lane < a.dim;
+    const bool in = 2 * lane < A.dim;
     for (int s = 0; s < A.splits; ++s) {
         const float2 ml = A.part_ml[s * rows + row];
         const float f = exp2_fast(ml.x - base);
         sum += f * ml.y;
         if (in) {
-            const float2 o = *reinterpret_cast<const float2*>(A.part_o + (s * rows + row) * a.dim + 2 * lane);
+            const float2 o = *reinterpret_cast<const float2*>(A.part_o + (s * rows + row) * A.dim + 2 * lane);
             x += f * o.x;
             y += f * o.y;
         }
     }
     const int64_t pair = row / A.rows;
-    const int m = (int)(row - pair * A.rows), i = m / A.group;
-    const int n = (int)(pair / a.kv_heads), head = (int)(pair - (int64_t)n * a.kv_heads) * A.group + m - i * A.group;
+    const int m = (int)(row - pair * A.rows), i = step_of(A, m);
+    const int n = (int)(pair / A.kv_heads), head = (int)(pair - (int64_t)n * A.kv_heads) * A.group + m - i * A.group;
     const float f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-    T* const to = static_cast<T*>(a.out) + n * a.out_strides[0] + i * a.out_strides[1] + head * a.out_strides[2];
+    T* const to = A.out.at<T>(n, i, head);
     if (in) {
         to[2 * lane] = (T)(x * f);
         to[2 * lane + 1] = (T)(y * f);
     }
-    if (a.stats && lane == 0)
-        reinterpret_cast<float2*>(a.stats)[((int64_t)n * a.heads + head) * a.q_steps + i] = make_float2(top, sum);
+    if (A.stats && lane == 0) A.stats[((int64_t)n * A.heads + head) * A.q_steps + i] = make_float2(top, sum);
 }
 
-// dbias from the row tiles' parts [count][columns]: block (x, y) sums rows y, y + gridDim.y, ... of 64 columns, then the
+// dbias from the blocks' parts [count][columns]: block (x, y) sums rows y, y + gridDim.y, ... of 64 columns, then the
 // second launch (one row of blocks) the sums. Fixed order.
 __global__ void __launch_bounds__(256) k_bias_sum(const float* parts, int count, int columns, float* sums, void* out, int type) {
     __shared__ float part[4][64];
@@ -212,7 +254,8 @@ __global__ void __launch_bounds__(256) k_bias_sum(const float* parts, int count,
 // ---------------------------------------------------------------- host
 
 bool aligned(const void* p, const int64_t* strides) {
-    return p && ((uintptr_t)p & 15) == 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0;
+    return p && ((uintptr_t)p & 15) == 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0 &&
+           strides[1] >= 0 && strides[2] >= 0 && strides[1] < (1 << 24) && strides[2] < (1 << 24);
 }
 
 constexpr int kWavesWanted = 2048;  // waves that fill the chip: 256 CUs x 4 SIMDs x 2
@@ -228,11 +271,40 @@ int check_sizes(const GoiAttention* a, AttnRun* A, const char* who) {
     if (a->type != GOI_BF16 && a->type != GOI_F16) return policy_error(GOI_E_UNSUPPORTED, "%s: type is neither bf16 nor f16", who);
     if (a->dim < 8 || a->dim > 128 || a->dim % 8)
         return policy_error(GOI_E_UNSUPPORTED, "%s: dim %d is no multiple of 8 within 8 .. 128", who, a->dim);
-    A->a = *a;
+    const auto view = [](const void* p, const int64_t* s) {
+        return View{static_cast<char*>(const_cast<void*>(p)), s[0] * 2, (int32_t)s[1] * 2, (int32_t)s[2] * 2};
+    };
+    *A = AttnRun{};
+    A->q = view(a->q, a->q_strides);
+    A->k = view(a->k, a->k_strides);
+    A->v = view(a->v, a->v_strides);
+    A->out = view(a->out, a->out_strides);
+    A->dout = view(a->dout, a->dout_strides);
+    A->dq = view(a->dq, a->dq_strides);
+    A->dk = view(a->dk, a->dk_strides);
+    A->dv = view(a->dv, a->dv_strides);
+    A->bias = a->bias;
+    A->buckets = a->buckets;
+    A->first = a->first;
+    A->lengths = a->lengths;
+    A->stats = reinterpret_cast<float2*>(a->stats);
+    A->n_worlds = a->n_worlds;
+    A->q_steps = a->q_steps;
+    A->k_steps = a->k_steps;
+    A->heads = a->heads;
+    A->kv_heads = a->kv_heads;
+    A->dim = a->dim;
+    A->causal = a->causal;
+    A->n_buckets = a->n_buckets;
+    A->n_distances = a->bias ? a->n_distances : 1;
+    A->bias_type = a->bias_type;
+    A->type = a->type;
+    A->scale = a->scale;
     A->group = a->heads / a->kv_heads;
+    A->group_magic = A->group > 1 ? (uint32_t)(((1ull << 32) + A->group - 1) / A->group) : 0;
     const int64_t rows = (int64_t)a->q_steps * A->group;
-    if (rows > INT_MAX - 256 || a->k_steps > INT_MAX - 256 || (int64_t)a->n_worlds * a->heads > INT_MAX)
-        return policy_error(GOI_E_UNSUPPORTED, "%s: sizes above 31 bits", who);
+    if (rows > INT_MAX - 256 || rows * A->group >= (1ll << 32) || a->k_steps > INT_MAX - 256 || (int64_t)a->n_worlds * a->heads > INT_MAX)
+        return policy_error(GOI_E_UNSUPPORTED, "%s: sizes above 31 bits, or q_steps * group^2 above 32", who);
     if (a->bias) {
         if (!a->buckets) return policy_error(GOI_E_ARG, "%s: a bias without buckets", who);
         if (a->n_buckets < 1 || a->n_distances < 1) return policy_error(GOI_E_ARG, "%s: an empty bias", who);
@@ -240,32 +312,36 @@ int check_sizes(const GoiAttention* a, AttnRun* A, const char* who) {
             return policy_error(GOI_E_UNSUPPORTED, "%s: the bias is of another 16-bit type", who);
         if (!a->causal && a->n_distances % 2 == 0)
             return policy_error(GOI_E_SHAPE, "%s: without a causal order buckets holds both directions and distance 0", who);
-        if (a->n_buckets > kMaxBuckets || (int64_t)A->group * a->n_distances > kMaxBiasTable)
-            return policy_error(GOI_E_UNSUPPORTED, "%s: more than %d buckets, or group * n_distances above %d", who, kMaxBuckets,
-                                kMaxBiasTable);
+        if (a->n_buckets > kMaxBuckets || (int64_t)A->group * (a->n_distances + 2 * kPad) > kMaxBiasTable)
+            return policy_error(GOI_E_UNSUPPORTED, "%s: more than %d buckets, or group * (n_distances + %d) above %d", who,
+                                kMaxBuckets, 2 * kPad, kMaxBiasTable);
     }
     A->rows = (int)rows;
     A->blocks = (A->rows + 31) / 32;
-    A->origin = a->causal ? 0 : (a->n_distances - 1) / 2;
+    A->origin = a->causal ? 0 : (A->n_distances - 1) / 2;
+    A->table = A->n_distances + 2 * kPad;
     A->c = a->scale * kLog2e;
     A->splits = 1;
-    A->span = 0;
-    A->part_o = nullptr;
-    A->part_ml = nullptr;
-    A->row_info = nullptr;
-    A->block_info = nullptr;
-    A->part_bias = nullptr;
     return GOI_OK;
 }
 
-int check_grid(int64_t blocks, const char* who) {
-    return blocks > INT_MAX ? policy_error(GOI_E_UNSUPPORTED, "%s: more than 2^31 blocks", who) : GOI_OK;
+// The items of a key head and the blocks that share them. Short windows: a block stages the bias once for many items, so the
+// blocks are those that the chip holds a few times over; long ones, whose items differ in size, go to blocks of their own.
+constexpr int kCus = 256, kCuLds = 160 * 1024;  // MI355X
+int share_items(AttnRun* A, int64_t items, int waves, size_t lds, const char* who, bool apart = false) {
+    const int64_t resident = kCus * std::max<int64_t>(1, std::min<int64_t>(8 / waves, kCuLds / (int64_t)(lds + 512)));
+    const int64_t want = A->k_steps >= 1024 || apart ? items : std::max<int64_t>(1, 3 * resident / A->kv_heads);
+    const int64_t blocks = std::min(items, want);
+    if (items > INT_MAX || blocks * A->kv_heads > INT_MAX) return policy_error(GOI_E_UNSUPPORTED, "%s: more than 2^31 tiles", who);
+    A->items = (int)items;
+    A->per_head = (int)blocks;
+    return GOI_OK;
 }
 
 // The key axis is split where the row tiles alone would leave the chip mostly idle: into as many ranges of at least 128 keys
 // as bring the waves to kWavesWanted.
 void plan_forward(AttnRun* A, int* waves) {
-    const GoiAttention& a = A->a;
+    const AttnRun& a = *A;
     *waves = waves_for(A->rows);
     A->tiles = (A->rows + 32 * *waves - 1) / (32 * *waves);
     const int64_t blocks = (int64_t)a.n_worlds * a.kv_heads * A->tiles;
@@ -281,42 +357,45 @@ uint64_t round16(uint64_t x) { return (x + 15) & ~(uint64_t)15; }
 
 uint64_t forward_bytes(const AttnRun& A) {
     if (A.splits <= 1) return 0;
-    const uint64_t rows = (uint64_t)A.a.n_worlds * A.a.kv_heads * A.rows * A.splits;
-    return round16(rows * sizeof(float2)) + rows * A.a.dim * sizeof(float);
+    const uint64_t rows = (uint64_t)A.n_worlds * A.kv_heads * A.rows * A.splits;
+    return round16(rows * sizeof(float2)) + rows * A.dim * sizeof(float);
 }
 
 // The backward scratch: row and block infos, dbias' parts and their first sums.
 constexpr int kBiasSums = 128;
 struct BackwardPlan {
-    int waves, tiles;
+    int waves;
     uint64_t blocks_at, parts_at, sums_at, bytes;
-    int64_t parts;
 };
-BackwardPlan plan_backward(const AttnRun& A) {
-    BackwardPlan p;
-    const GoiAttention& a = A.a;
+// Fills in the launch of the pass over rows
+int plan_backward(AttnRun* run, BackwardPlan* plan, const char* who) {
+    BackwardPlan& p = *plan;
+    AttnRun& A = *run;
+    const AttnRun& a = A;
     p.waves = waves_for(A.rows);
-    p.tiles = (A.rows + 32 * p.waves - 1) / (32 * p.waves);
+    A.tiles = (A.rows + 32 * p.waves - 1) / (32 * p.waves);
+    // the bias' sums of a lane are of one head: items whose rows start at other heads are kept apart
+    const int rc = share_items(run, (int64_t)a.n_worlds * A.tiles, p.waves, attention_dq_lds(A, p.waves), who,
+                               a.bias && 32 % A.group != 0);
+    if (rc != GOI_OK) return rc;
     const uint64_t pairs = (uint64_t)a.n_worlds * a.kv_heads;
     p.blocks_at = round16(pairs * A.rows * sizeof(RowInfo));
     p.parts_at = round16(p.blocks_at + pairs * A.blocks * sizeof(BlockInfo));
-    p.parts = (int64_t)a.n_worlds * p.tiles;
     const uint64_t columns = a.bias ? (uint64_t)a.heads * a.n_buckets : 0;
-    p.sums_at = round16(p.parts_at + p.parts * columns * sizeof(float));
+    p.sums_at = round16(p.parts_at + A.per_head * columns * sizeof(float));
     p.bytes = p.sums_at + kBiasSums * columns * sizeof(float);
-    return p;
+    return GOI_OK;
 }
 
 template <typename T, int DP, int NW>
 hipError_t launch_forward(const AttnRun& A, hipStream_t st) {
-    constexpr int KT = NW == 1 && DP == 128 ? 32 : 64, NBUF = NW == 1 ? 1 : 2;
-    const size_t lds = NBUF * 2 * KT * DP * sizeof(T) + (A.a.bias ? (size_t)A.group * A.a.n_distances * sizeof(float) : 0);
-    const dim3 grid((unsigned)((int64_t)A.a.n_worlds * A.a.kv_heads * A.tiles * A.splits)), block(64 * NW);
+    const size_t lds = attention_lds(A, NW);
+    const dim3 grid((unsigned)(A.kv_heads * A.per_head)), block(64 * NW);
     if (A.splits > 1) {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention<T, DP, NW, true>),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL((k_attention<T, DP, NW, true>), grid, block, lds, st, A);
-        const int64_t rows = (int64_t)A.a.n_worlds * A.a.kv_heads * A.rows;
+        const int64_t rows = (int64_t)A.n_worlds * A.kv_heads * A.rows;
         hipLaunchKernelGGL(k_attention_join<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, A);
     } else {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention<T, DP, NW, false>),
@@ -334,14 +413,12 @@ hipError_t launch_forward(const AttnRun& A, int waves, hipStream_t st) {
 
 template <typename T>
 hipError_t launch_forward(const AttnRun& A, int waves, hipStream_t st) {
-    const int dp = attention_dim_tile(A.a.dim);
+    const int dp = attention_dim_tile(A.dim);
     return dp == 32 ? launch_forward<T, 32>(A, waves, st) : dp == 64 ? launch_forward<T, 64>(A, waves, st)
                                                                     : launch_forward<T, 128>(A, waves, st);
 }
 
 }  // namespace
-
-int attention_dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 }  // namespace goi
 
@@ -355,7 +432,10 @@ int32_t goi_attention_workspace(const GoiAttention* a, int32_t backward, uint64_
     const int rc = check_sizes(a, &A, "goi_attention_workspace");
     if (rc != GOI_OK) return rc;
     if (backward) {
-        *bytes = plan_backward(A).bytes;
+        BackwardPlan p;
+        const int rc = plan_backward(&A, &p, "goi_attention_workspace");
+        if (rc != GOI_OK) return rc;
+        *bytes = p.bytes;
     } else {
         int waves;
         plan_forward(&A, &waves);
@@ -377,7 +457,7 @@ int32_t goi_attention_forward(const GoiAttention* a, void* workspace, uint64_t w
     plan_forward(&A, &waves);
     if (forward_bytes(A) > workspace_bytes || (forward_bytes(A) && (!workspace || (uintptr_t)workspace & 15)))
         return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
-    rc = check_grid((int64_t)a->n_worlds * a->kv_heads * A.tiles * A.splits, who);
+    rc = share_items(&A, (int64_t)a->n_worlds * A.tiles * A.splits, waves, attention_lds(A, waves), who);
     if (rc != GOI_OK) return rc;
     if (A.splits > 1) {
         const uint64_t rows = (uint64_t)a->n_worlds * a->kv_heads * A.rows * A.splits;
@@ -402,25 +482,24 @@ int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t 
         (keys && (!aligned(a->k, a->k_strides) || !aligned(a->v, a->v_strides) || !aligned(a->dk, a->dk_strides) ||
                   !aligned(a->dv, a->dv_strides))))
         return policy_error(GOI_E_ARG, "%s: a null or misaligned tensor (16-byte pointers, strides of 8 elements)", who);
-    const BackwardPlan p = plan_backward(A);
+    BackwardPlan p;
+    rc = plan_backward(&A, &p, who);
+    if (rc != GOI_OK) return rc;
     if (p.bytes > workspace_bytes || (p.bytes && (!workspace || (uintptr_t)workspace & 15)))
         return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
     const int64_t pairs = (int64_t)a->n_worlds * a->kv_heads;
-    rc = check_grid(pairs * std::max<int64_t>(p.tiles, (a->k_steps + 31) / 32), who);
-    if (rc != GOI_OK) return rc;
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
     char* const ws = static_cast<char*>(workspace);
     A.row_info = reinterpret_cast<RowInfo*>(ws);
     A.block_info = reinterpret_cast<BlockInfo*>(ws + p.blocks_at);
     A.part_bias = reinterpret_cast<float*>(ws + p.parts_at);
-    A.tiles = p.tiles;
     hipError_t e = hipSuccess;
     if (rows) e = launch_attention_dq(A, p.waves, st);
     if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
     if (a->bias) {
         const int columns = a->heads * a->n_buckets, x = (columns + 63) / 64;
         float* const sums = reinterpret_cast<float*>(ws + p.sums_at);
-        const int count = rows ? (int)p.parts : 0, y = std::max(1, std::min(kBiasSums, (count + 3) / 4));
+        const int count = rows ? A.per_head : 0, y = std::max(1, std::min(kBiasSums, (count + 3) / 4));
         if (y > 1)
             hipLaunchKernelGGL(k_bias_sum, dim3(x, y), dim3(256), 0, st, A.part_bias, count, columns, sums, nullptr, 0);
         hipLaunchKernelGGL(k_bias_sum, dim3(x, 1), dim3(256), 0, st, y > 1 ? sums : A.part_bias, y > 1 ? y : count, columns,
@@ -430,9 +509,12 @@ int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t 
     }
     if (keys) {
         // keys of 32 a wave: fewer waves a block where blocks of 4 would not fill the chip
-        int waves = waves_for(a->k_steps);
-        while (waves > 1 && pairs * ((a->k_steps + 32 * waves - 1) / (32 * waves)) < 512) waves /= 2;
+        const int least = attention_dim_tile(a->dim) == 128 ? 2 : 1;
+        int waves = std::max(least, waves_for(a->k_steps));
+        while (waves > least && pairs * ((a->k_steps + 32 * waves - 1) / (32 * waves)) < 512) waves /= 2;
         A.tiles = (a->k_steps + 32 * waves - 1) / (32 * waves);
+        rc = share_items(&A, (int64_t)a->n_worlds * A.tiles, waves, attention_lds(A, waves), who);
+        if (rc != GOI_OK) return rc;
         e = launch_attention_dkv(A, waves, st);
         if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
     }

@@ -3,9 +3,9 @@
 //
 // The query heads that share a key head are packed with the steps into one axis of rows, row m = step m / group, head
 // m % group of the key head's group, so a tile of rows fills whatever the two numbers are, and each key is read once for
-// all of its heads. Scores are computed transposed, keys x rows: a lane of the 32 x 32 product then holds 16 keys of ONE
-// row, so that the softmax runs within a lane (and its partner 32 lanes away), and the probabilities, rounded, are the
-// second operand of the product with the values as they stand.
+// all of its heads. The forward pass and the pass over rows compute scores transposed, keys x rows: a lane of the 32 x 32
+// product then holds 16 keys of ONE row, so that the softmax runs within a lane (and its partner 32 lanes away), and the
+// probabilities, rounded, are the second operand of the product with the values as they stand.
 #pragma once
 
 #include <climits>
@@ -16,7 +16,9 @@
 namespace goi {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxBuckets = 64, kMaxBiasTable = 4096;
+constexpr int kMaxBuckets = 64, kMaxBiasTable = 6144;
+constexpr int kPad = 64;       // entries before and after a head's bias table (stage_bias)
+constexpr int kSumPitch = 65;  // words from one bucket's sums to the next's (policy_attention_dq.hip)
 
 // A row's part of what the backward kernels hand over: its largest score in powers of two (+infinity for a row without keys,
 // so that exp2(s - top) is 0), the inverse of its sum, delta = out . dout times that, and the keys it sees.
@@ -24,91 +26,169 @@ struct RowInfo {
     float top, inv, delta;
     int lo, hi;
 };
-// The same for 32 rows: the keys that any row sees [lo, hi), those that every row sees [full_lo, full_hi), and the range
-// of the rows' positions plus origin.
+// The same for 32 rows: the keys that any row sees lie in [lo, hi), those that every row sees are [full_lo, full_hi), and the
+// range of the rows' positions plus origin.
 struct BlockInfo {
-    int lo, hi, full_lo, full_hi, pos_lo, pos_hi, pad0, pad1;
+    int lo, hi, full_lo, full_hi, pos_lo, pos_hi;
+    int awake;  // every row sees a key
+    int pad;
+};
+
+// A tensor [world, step, head, dim]: strides in bytes
+struct View {
+    char* p;
+    int64_t world;
+    int32_t step, head;
+    template <typename T>
+    __device__ __forceinline__ T* at(int n, int i, int h) const {
+        return reinterpret_cast<T*>(p + n * world + (int64_t)i * step + (int64_t)h * head);
+    }
 };
 
 struct AttnRun {
-    GoiAttention a;
-    int group;   // query heads per key head
-    int rows;    // packed rows of a key head: q_steps * group
-    int tiles;   // row tiles (forward, dq) or key tiles (dkv) of a key head
+    View q, k, v, out, dout, dq, dk, dv;
+    const void* bias;
+    const int32_t *buckets, *first, *lengths;
+    float2* stats;
+    int n_worlds, q_steps, k_steps, heads, kv_heads, dim, causal, n_buckets, n_distances, bias_type, type;
+    float scale, c;       // c = scale * log2(e)
+    int group;            // query heads per key head
+    uint32_t group_magic; // ceil(2^32 / group), 0 for 1
+    int rows;             // packed rows of a key head: q_steps * group
+    int blocks;           // 32-row blocks of a key head
+    int tiles;            // row tiles (forward, dq) or key tiles (dkv) of a key head
+    int items;            // tiles (and splits) of all the worlds' windows with one key head, shared out over `per_head` blocks
+    int per_head;
     int splits;  // forward: the key axis is cut into `splits` ranges of `span` keys, joined afterwards
     int span;
     int origin;  // index of distance 0 in buckets
-    int blocks;  // 32-row blocks of a key head
-    float c;     // scale * log2(e)
-    float* part_o;   // forward, splits > 1: [splits][world, key head, row][dim] unnormalised outputs
-    float2* part_ml; // and [splits][world, key head, row] maximum (powers of two) and sum
+    int table;   // entries of a head's bias table in LDS: n_distances + 2 kPad
+    float* part_o;          // forward, splits > 1: [splits][world, key head, row][dim] unnormalised outputs
+    float2* part_ml;        // and [splits][world, key head, row] maximum (powers of two) and sum
     RowInfo* row_info;      // backward: [world, key head][rows]
     BlockInfo* block_info;  // [world, key head][blocks]
-    float* part_bias;       // [world, row tile][heads * n_buckets]
+    float* part_bias;       // [block of a key head][heads * n_buckets]
 };
 
-// Host side (policy_attention.hip): checks, sizes and launches.
+// ---- host side (policy_attention.hip: checks, sizes and launches)
+
+inline int attention_dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+// Rows of a tile in LDS: 64, or 32 of 128 elements or for a single wave, so that two blocks' double buffers fit a CU and a
+// thread holds few chunks of the next tile. Two tiles of LDS for blocks of several waves; a single wave needs no barrier and
+// overwrites its own.
+constexpr int tile_rows(int dp, int waves) { return dp == 128 || waves == 1 ? 32 : 64; }
+constexpr int tile_buffers(int waves) { return waves == 1 ? 1 : 2; }
+inline size_t attention_lds(const AttnRun& A, int waves) {
+    const int dp = attention_dim_tile(A.dim);
+    return (size_t)tile_buffers(waves) * 2 * tile_rows(dp, waves) * dp * 2 + (A.bias ? (size_t)A.group * A.table * sizeof(float) : 0);
+}
+inline size_t attention_dq_lds(const AttnRun& A, int waves) {
+    return attention_lds(A, waves) +
+           (A.bias ? (size_t)waves * A.n_buckets * kSumPitch * sizeof(float) + (size_t)A.table * 2 : 0);
+}
+
 hipError_t launch_attention_dq(const AttnRun& A, int waves, hipStream_t st);
 hipError_t launch_attention_dkv(const AttnRun& A, int waves, hipStream_t st);
-int attention_dim_tile(int dim);  // 32, 64 or 128
+
+// ---- device side
+
+// m / group: exact while m * group < 2^32 (checked on the host)
+__device__ __forceinline__ int step_of(const AttnRun& A, int m) {
+    return A.group_magic ? (int)__umulhi((uint32_t)m, A.group_magic) : m;
+}
 
 __device__ __forceinline__ int history(const AttnRun& A, int n) {
-    return A.a.lengths ? min(max(A.a.lengths[n], 0), A.a.k_steps) : A.a.k_steps;
+    return A.lengths ? min(max(A.lengths[n], 0), A.k_steps) : A.k_steps;
 }
 
 struct Row {
-    bool valid;    // m < rows
-    int i, hl;     // step and head within the group
-    int pos;       // position + origin
-    int lo, hi;    // keys seen; lo = hi = 0 if none
+    bool valid;  // m < rows
+    int i, hl;   // step and head within the group
+    int pos;     // position + origin
+    int lo, hi;  // keys seen; lo = hi = 0 if none
 };
 
 __device__ __forceinline__ Row make_row(const AttnRun& A, int n, int L, int m) {
     Row r;
     r.valid = m < A.rows;
-    r.i = r.valid ? m / A.group : 0;
+    r.i = r.valid ? step_of(A, m) : 0;
     r.hl = r.valid ? m - r.i * A.group : 0;
-    const int p = L - A.a.q_steps + r.i;
+    const int p = L - A.q_steps + r.i;
     r.pos = p + A.origin;
-    r.lo = A.a.first ? max(A.a.first[(int64_t)n * A.a.q_steps + r.i], 0) : 0;
-    r.hi = A.a.causal ? min(p + 1, L) : L;
+    r.lo = A.first ? max(A.first[(int64_t)n * A.q_steps + r.i], 0) : 0;
+    r.hi = A.causal ? min(p + 1, L) : L;
     if (!r.valid || r.hi <= r.lo) r.lo = r.hi = 0;
     return r;
 }
 
-__device__ __forceinline__ BlockInfo make_block(const Row& r) {
+// Of the 32 rows from m0 on, which the wave's lanes hold twice. Positions, and with them the ends of the ranges of keys, rise
+// with the row, so where no row sleeps only the ranges' beginnings are compared.
+__device__ __forceinline__ BlockInfo make_block(const AttnRun& A, int L, int m0, const Row& r) {
     BlockInfo b;
-    b.lo = wave_min(r.hi > r.lo ? r.lo : INT_MAX);
-    b.hi = wave_max(r.hi);
-    b.full_lo = wave_max(r.valid ? r.lo : 0);
-    b.full_hi = wave_min(r.valid ? r.hi : INT_MAX);
-    b.pos_lo = wave_min(r.valid ? r.pos : INT_MAX);
-    b.pos_hi = wave_max(r.valid ? r.pos : INT_MIN);
-    b.pad0 = b.pad1 = 0;
+    const int first = L - A.q_steps + step_of(A, min(m0, A.rows - 1));
+    const int last = L - A.q_steps + step_of(A, min(m0 + 31, A.rows - 1));
+    b.pos_lo = first + A.origin;
+    b.pos_hi = last + A.origin;
+    b.awake = __all(!r.valid || r.hi > r.lo);
+    const bool any = __any(r.hi > r.lo);
+    b.hi = !any ? 0 : A.causal ? min(last + 1, L) : L;
+    b.full_hi = !b.awake ? 0 : A.causal ? min(first + 1, L) : L;
+    if (any && !b.awake) b.hi = wave_max(r.hi);
+    b.lo = any ? 0 : INT_MAX;
+    b.full_lo = 0;
+    if (A.first) {
+        b.lo = wave_min(r.hi > r.lo ? r.lo : INT_MAX);
+        b.full_lo = wave_max(r.valid ? r.lo : 0);
+    }
+    b.pad = 0;
     return b;
 }
 
-// ROWS rows of `dim` elements on their way to an LDS tile: load() issues the loads (of addresses inside the tensor, whatever
-// the row), store() writes the tile with zeros in the rows outside [lo, hi) and past dim.
+// ROWS rows of a tensor on their way to an LDS tile: load() issues the loads (inside the tensor, whatever the row), store()
+// writes the tile with zeros in the rows from hi on and past dim. A thread's chunks keep their places in every tile, so a
+// whole tile's addresses are the tile's own (the same for every lane) and offsets computed once.
 template <typename T, int DP, int ROWS, int NT>
 struct KeyStage {
     static constexpr int N = ROWS * (DP / 8) / NT;
     static_assert(ROWS * (DP / 8) % NT == 0, "whole chunks a thread");
     int4_t x[N];
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int lo, int hi, int dim, int tid) {
+    uint32_t at[N];
+    const char* base;
+    int32_t stride;
+    int dim;
+    __device__ __forceinline__ static int row_of(int j, int tid) { return (tid + j * NT) / (DP / 8); }
+    __device__ __forceinline__ static int chunk_of(int j, int tid) { return (tid + j * NT) % (DP / 8); }
+    __device__ __forceinline__ KeyStage(const View& x, int n, int head, int d, int tid)
+        : base(x.at<char>(n, 0, head)), stride(x.step), dim(d) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int c = tid + j * NT, row = c / (DP / 8), ch = c % (DP / 8);
-            const int key = min(max(row0 + row, lo), hi - 1);
-            x[j] = *reinterpret_cast<const int4_t*>(base + key * stride + (ch * 8 < dim ? ch * 8 : 0));
+        for (int j = 0; j < N; ++j)
+            at[j] = (uint32_t)row_of(j, tid) * (uint32_t)stride + (chunk_of(j, tid) * 8 < dim ? chunk_of(j, tid) * 16 : 0);
+    }
+    __device__ __forceinline__ void load(int row0, int hi, int tid) {
+        const char* const from = base + (int64_t)row0 * stride;
+        if (row0 + ROWS <= hi) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = *reinterpret_cast<const int4_t*>(from + at[j]);
+        } else {
+            const int last = hi - 1 - row0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int over = max(row_of(j, tid) - last, 0);
+                x[j] = *reinterpret_cast<const int4_t*>(from + (at[j] - (uint32_t)over * (uint32_t)stride));
+            }
         }
     }
-    __device__ __forceinline__ void store(T* tile, int row0, int lo, int hi, int dim, int tid) const {
+    __device__ __forceinline__ void store(T* tile, int row0, int hi, int tid) const {
+        if (row0 + ROWS <= hi && dim == DP) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int c = tid + j * NT, row = c / (DP / 8), ch = c % (DP / 8);
-            const bool in = row0 + row >= lo && row0 + row < hi && ch * 8 < dim;
-            reinterpret_cast<int4_t*>(tile)[chunk_at<DP>(row, ch)] = in ? x[j] : int4_t{0, 0, 0, 0};
+            for (int j = 0; j < N; ++j)
+                reinterpret_cast<int4_t*>(tile)[chunk_at<DP>(row_of(j, tid), chunk_of(j, tid))] = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const bool in = row0 + row_of(j, tid) < hi && chunk_of(j, tid) * 8 < dim;
+                reinterpret_cast<int4_t*>(tile)[chunk_at<DP>(row_of(j, tid), chunk_of(j, tid))] = in ? x[j] : int4_t{0, 0, 0, 0};
+            }
         }
     }
 };
@@ -129,13 +209,15 @@ __device__ __forceinline__ void load_operand(half8<T> (&f)[DP / 16], const T* ro
     }
 }
 
-// The bias table of key head g's group in LDS, [group][n_distances], in powers of two. Finite entries are held within
-// +-1.7e38, so that a type's lowest value, a usual mask, stays finite here and a row of such entries alone is still a row of
-// equal scores, as in the formula.
+// The bias table of key head g's group in LDS, [group][A.table], in powers of two. A head's entries are those of the distances
+// -kPad .. n_distances - 1 + kPad, each taken from the nearest end of the map where it lies outside: any pair of a 32 x 32 block
+// that is not all at one end (one_distance) finds its entry without clamping its distance, and the 16 pairs of a lane lie at fixed
+// places from one another. Finite entries are held within +-1.7e38, so that a type's lowest value, a usual mask, stays
+// finite here and a row of such entries alone is still a row of equal scores, as in the formula.
 __device__ __forceinline__ void stage_bias(const AttnRun& A, int g, float* table, int tid, int nt) {
-    const GoiAttention& a = A.a;
-    for (int x = tid; x < A.group * a.n_distances; x += nt) {
-        const int hl = x / a.n_distances, dist = x - hl * a.n_distances;
+    const AttnRun& a = A;
+    for (int x = tid; x < A.group * A.table; x += nt) {
+        const int hl = x / A.table, dist = min(max(x - hl * A.table - kPad, 0), a.n_distances - 1);
         const int b = min(max(a.buckets[dist], 0), a.n_buckets - 1);
         const int64_t at = (int64_t)(g * A.group + hl) * a.n_buckets + b;
         float v;
@@ -148,7 +230,7 @@ __device__ __forceinline__ void stage_bias(const AttnRun& A, int g, float* table
 }
 
 // The place in a table of n distances of every pair of a 32-key block at key0 with rows at positions pos_lo .. pos_hi, or -1
-// where it is not one place.
+// where it is not one place; every pair is then within 31 + (pos_hi - pos_lo) <= 62 of a place in the table.
 __device__ __forceinline__ int one_distance(int key0, int pos_lo, int pos_hi, int n) {
     const int a = min(max(pos_lo - (key0 + 31), 0), n - 1), b = min(max(pos_hi - key0, 0), n - 1);
     return a == b ? a : -1;
@@ -165,23 +247,19 @@ __device__ __forceinline__ float16_t raw_scores(const T* tile, int row0, const h
     return s;
 }
 
-// s * c + bias of the lane's 16 keys from key0 on (keys x rows layout). bias: the row's table, or null
+// s * c + bias of the lane's 16 keys from key0 on (keys x rows layout). bias: the entry of distance 0 of the row's table, or
+// null
 __device__ __forceinline__ void scale_scores(float16_t& s, float c, const float* bias, int n_dist, int key0, int pos,
                                              int pos_lo, int pos_hi, int half) {
-    if (!bias) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= c;
-        return;
-    }
-    const int one = one_distance(key0, pos_lo, pos_hi, n_dist);
+    const int one = bias ? one_distance(key0, pos_lo, pos_hi, n_dist) : 0;
     if (one >= 0) {
-        const float b = bias[one];
+        const float b = bias ? bias[one] : 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = s[r] * c + b;
     } else {
+        const float* const t = bias + (pos - key0 - 4 * half - 27);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            s[r] = s[r] * c + bias[min(max(pos - key0 - mfma_row(r, half), 0), n_dist - 1)];
+        for (int r = 0; r < 16; ++r) s[r] = s[r] * c + t[27 - mfma_row(r, 0)];
     }
 }
 
@@ -198,6 +276,48 @@ __device__ __forceinline__ void store_row(T* row, const float16_t (&o)[DP / 32],
             for (int e = 0; e < 4; ++e) y[e] = (T)(o[b][4 * x + e] * f);
             if (d < dim) *reinterpret_cast<half4<T>*>(row + d) = y;
         }
+}
+
+// ---- values that are not finite in blocks that some rows do not see
+//
+// A product takes 0 * NaN as NaN, so in a block where some pair is masked, a row of the tile that is not finite would reach
+// the sums of those that do not see it. Such blocks are looked through (finite_rows); a wave that found one computes its results
+// again at the end, pair by pair, with the pairs that do not count left out (careful_score and the loops that call it).
+
+// Whether all elements of 32 rows of a tile are finite: the largest exponent field among them is not all ones
+template <typename T, int DP>
+__device__ __forceinline__ bool finite_rows(const T* tile, int row0, int lane) {
+    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+    ushort2_t most = {0, 0};
+#pragma unroll
+    for (int j = 0; j < DP / 16; ++j) {  // 32 rows of DP / 8 chunks, in the order in which they lie
+        union {
+            int4_t v;
+            ushort2_t h[4];
+        } u;
+        u.v = reinterpret_cast<const int4_t*>(tile)[row0 * (DP / 8) + j * 64 + lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, u.h[e] & (unsigned short)0x7fff);
+    }
+    constexpr unsigned short kInf = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80 : 0x7c00;
+    return !__any(most[0] >= kInf || most[1] >= kInf);
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+    for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// Elements lane and lane + 64 of a row of dim elements (zeros past it)
+template <typename T>
+__device__ __forceinline__ float2 two_elements(const T* row, int dim, int lane) {
+    return make_float2(lane < dim ? (float)row[lane] : 0.0f, lane + 64 < dim ? (float)row[lane + 64] : 0.0f);
+}
+
+// The score of one pair in powers of two, from the whole wave: x and y its two rows as two_elements gives them
+__device__ __forceinline__ float careful_score(const AttnRun& A, float2 x, float2 y, const float* bias, int distance) {
+    const float s = wave_sum(x.x * y.x + x.y * y.y) * A.c;
+    return bias ? s + bias[min(max(distance + A.origin, 0), A.n_distances - 1)] : s;
 }
 
 template <int N>

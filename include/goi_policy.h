@@ -42,7 +42,7 @@ extern "C" {
  * probabilities and their gradients are rounded to the inputs' type for the second products.
  *
  * Limits: type GOI_BF16 or GOI_F16; dim a multiple of 8, 8 .. 128; 16-byte aligned pointers and strides (elements) that are
- * multiples of 8, the last axis contiguous; n_buckets <= 64; group * n_distances <= 4096. A bucket outside 0 .. n_buckets - 1 is
+ * multiples of 8 (steps and heads within 0 .. 2^24), the last axis contiguous; n_buckets <= 64; group * (n_distances + 128) <= 6144. A bucket outside 0 .. n_buckets - 1 is
  * taken as the nearest one. bias_type is type or GOI_F32. stats is [n_worlds, heads, q_steps, 2] contiguous and may be null in the
  * forward call. */
 typedef struct GoiAttention {

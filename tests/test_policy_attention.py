@@ -191,6 +191,38 @@ def test_rows_without_keys(waves):
 
 
 @gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("t", [30, 100])
+def test_values_that_only_some_rows_see(t, d, bad):
+    """A broken episode (values that are not finite) shares tiles with a sound one: it reaches the rows and keys of its own
+    episode only."""
+    n, h, g = 2, 4, 2
+    q, k, v, dout = tensors(n, t, t, h, g, d)
+    cut = t // 2 + 3
+    first = torch.zeros(n, t, dtype=torch.int32, device="cuda")
+    first[0, cut:] = cut
+    args = dict(first=first, **table(h))
+    clean = [x.clone() for x in (q, k, v, dout)]
+    for x in clean:
+        x[0, :cut] = 0
+    val, tol = reference(*clean[:3], dout=clean[3], **args)
+    q[0, 5, :, 3] = bad
+    k[0, 9, :, 1] = bad
+    v[0, 7, :, 2] = bad
+    dout[0, 11, :, 4] = bad
+    got = run_both(q, k, v, dout, **args)
+    assert not torch.isfinite(got["out"][0, 5]).any() and not torch.isfinite(got["out"][0, 7:cut, :, 2]).any()
+    for name in ("out", "dq", "dk", "dv"):
+        check({name: got[name][0, cut:]}, {name: val[name][0, cut:]}, {name: tol[name][0, cut:]})
+        check({name: got[name][1]}, {name: val[name][1]}, {name: tol[name][1]})
+        if name != "out":
+            assert not torch.isfinite(got[name][0, :cut].float()).all(), name
+    one_step = policy.attention(q[:, -1:], k, v, first=first[:, -1:].contiguous(), **table(h))
+    check({"out": one_step}, {"out": val["out"][:, -1:]}, {"out": tol["out"][:, -1:]})
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("n,tk,h,g,d", [(1, 1, 4, 1, 64), (3, 60, 8, 2, 64), (40, 130, 4, 4, 32), (2, 5000, 8, 1, 128),
                                         (1, 40000, 16, 2, 64), (5, 700, 12, 4, 80)])
@@ -382,7 +414,7 @@ def _call(name, **fields):
     (dict(kv_heads=0), abi.GOI_E_ARG, "no heads"), (dict(q=None), abi.GOI_E_ARG, "null"), (dict(v=4104), abi.GOI_E_ARG, "misaligned"),
     (dict(k_strides=(4, 8, 8)), abi.GOI_E_ARG, "misaligned"), (dict(bias=4096), abi.GOI_E_ARG, "buckets"),
     (dict(bias=4096, buckets=4096, n_buckets=65, n_distances=9, bias_type=abi.BF16), abi.GOI_E_UNSUPPORTED, "65|buckets"),
-    (dict(bias=4096, buckets=4096, n_buckets=9, n_distances=2049, bias_type=abi.BF16), abi.GOI_E_UNSUPPORTED, "4096"),
+    (dict(bias=4096, buckets=4096, n_buckets=9, n_distances=4000, bias_type=abi.BF16), abi.GOI_E_UNSUPPORTED, "6144"),
     (dict(bias=4096, buckets=4096, n_buckets=9, n_distances=9, bias_type=abi.F16), abi.GOI_E_UNSUPPORTED, "16-bit"),
     (dict(bias=4096, buckets=4096, n_buckets=9, n_distances=8, causal=0), abi.GOI_E_SHAPE, "both directions"),
     (dict(q_steps=1 << 30, heads=8), abi.GOI_E_UNSUPPORTED, "31 bits"),
