@@ -46,23 +46,37 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int range[2][NW];
     T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][keys, values][KT][DP]
-    float* const table = reinterpret_cast<float*>(lds + NBUF * 2 * KT * DP * sizeof(T));
+    const BiasLds bl(A, lds + NBUF * 2 * KT * DP * sizeof(T));
+    const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
     const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
-    if (A.bias) stage_bias(A, g, table, tid, NT);
-    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    for (int item = (int)((int64_t)block * A.items / A.per_head); item < end; ++item) {
-        // the later row tiles of a causal window see the most keys: they go first
-        int n = item / A.tiles, split = 0;
-        const int tile = A.tiles - 1 - (item - n * A.tiles);
+    if (A.bias) bl.stage(A, g, tid, NT);
+    // the later row tiles of a causal window see the most keys: they go first
+    const auto place_of = [&](int item, int* split, int* tile) {
+        int n = item / A.tiles;
+        *tile = A.tiles - 1 - (item - n * A.tiles);
+        *split = 0;
         if (kSplit) {
             const int x = n / A.splits;
-            split = n - x * A.splits;
+            *split = n - x * A.splits;
             n = x;
         }
-        const int L = history(A, n), m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
-        Row row = make_row(A, n, L, m);
+        return n;
+    };
+    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
+    int item = (int)((int64_t)block * A.items / A.per_head), split, tile;
+    int n = place_of(item, &split, &tile);
+    Ahead ahead = look_ahead(A, n, (tile * NW + wave) * 32 + (lane & 31));
+    for (; item < end; ++item) {
+        n = place_of(item, &split, &tile);
+        const int L = ahead.length, m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
+        Row row = make_row(A, ahead, m);
+        if (item + 1 < end) {
+            int s, t;
+            const int next = place_of(item + 1, &s, &t);
+            ahead = look_ahead(A, next, (t * NW + wave) * 32 + (lane & 31));
+        }
         if (kSplit) {
             row.lo = max(row.lo, split * A.span);
             row.hi = min(row.hi, (split + 1) * A.span);
@@ -84,7 +98,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
         const int head = g * A.group + row.hl;
         half8<T> q[DP / 16];
         load_operand<T, DP>(q, A.q.at<T>(n, row.i, head), row.valid, A.dim, lane);
-        __syncthreads();
+        if (NW > 1) __syncthreads();
         int lo = blk.lo, hi = blk.hi;  // the keys that some row of the block sees
         if constexpr (NW > 1) {
             lo = INT_MAX;
@@ -373,6 +387,7 @@ int plan_backward(AttnRun* run, BackwardPlan* plan, const char* who) {
     AttnRun& A = *run;
     const AttnRun& a = A;
     p.waves = waves_for(A.rows);
+    while (p.waves > 1 && attention_dq_lds(A, p.waves) > (size_t)kCuLds - 512) p.waves /= 2;
     A.tiles = (A.rows + 32 * p.waves - 1) / (32 * p.waves);
     // the bias' sums of a lane are of one head: items whose rows start at other heads are kept apart
     const int rc = share_items(run, (int64_t)a.n_worlds * A.tiles, p.waves, attention_dq_lds(A, p.waves), who,

@@ -18,7 +18,6 @@ namespace goi {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBuckets = 64, kMaxBiasTable = 6144;
 constexpr int kPad = 64;       // entries before and after a head's bias table (stage_bias)
-constexpr int kSumPitch = 65;  // words from one bucket's sums to the next's (policy_attention_dq.hip)
 
 // A row's part of what the backward kernels hand over: its largest score in powers of two (+infinity for a row without keys,
 // so that exp2(s - top) is 0), the inverse of its sum, delta = out . dout times that, and the keys it sees.
@@ -78,15 +77,6 @@ inline int attention_dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 
 // overwrites its own.
 constexpr int tile_rows(int dp, int waves) { return dp == 128 || waves == 1 ? 32 : 64; }
 constexpr int tile_buffers(int waves) { return waves == 1 ? 1 : 2; }
-inline size_t attention_lds(const AttnRun& A, int waves) {
-    const int dp = attention_dim_tile(A.dim);
-    return (size_t)tile_buffers(waves) * 2 * tile_rows(dp, waves) * dp * 2 + (A.bias ? (size_t)A.group * A.table * sizeof(float) : 0);
-}
-inline size_t attention_dq_lds(const AttnRun& A, int waves) {
-    return attention_lds(A, waves) +
-           (A.bias ? (size_t)waves * A.n_buckets * kSumPitch * sizeof(float) + (size_t)A.table * 2 : 0);
-}
-
 hipError_t launch_attention_dq(const AttnRun& A, int waves, hipStream_t st);
 hipError_t launch_attention_dkv(const AttnRun& A, int waves, hipStream_t st);
 
@@ -108,15 +98,26 @@ struct Row {
     int lo, hi;  // keys seen; lo = hi = 0 if none
 };
 
-__device__ __forceinline__ Row make_row(const AttnRun& A, int n, int L, int m) {
+// What a row's range of keys is made of: loaded an item ahead, so that the item's other loads wait for nothing
+struct Ahead {
+    int length, first;
+};
+__device__ __forceinline__ Ahead look_ahead(const AttnRun& A, int n, int m) {
+    Ahead x;
+    x.length = history(A, n);
+    x.first = A.first ? A.first[(int64_t)n * A.q_steps + step_of(A, min(m, A.rows - 1))] : 0;
+    return x;
+}
+
+__device__ __forceinline__ Row make_row(const AttnRun& A, const Ahead& x, int m) {
     Row r;
     r.valid = m < A.rows;
     r.i = r.valid ? step_of(A, m) : 0;
     r.hl = r.valid ? m - r.i * A.group : 0;
-    const int p = L - A.q_steps + r.i;
+    const int p = x.length - A.q_steps + r.i;
     r.pos = p + A.origin;
-    r.lo = A.first ? max(A.first[(int64_t)n * A.q_steps + r.i], 0) : 0;
-    r.hi = A.causal ? min(p + 1, L) : L;
+    r.lo = max(x.first, 0);
+    r.hi = A.causal ? min(p + 1, x.length) : x.length;
     if (!r.valid || r.hi <= r.lo) r.lo = r.hi = 0;
     return r;
 }
@@ -209,24 +210,50 @@ __device__ __forceinline__ void load_operand(half8<T> (&f)[DP / 16], const T* ro
     }
 }
 
-// The bias table of key head g's group in LDS, [group][A.table], in powers of two. A head's entries are those of the distances
+// The bias of key head g's group in LDS. table [group][A.table], in powers of two: a head's entries are those of the distances
 // -kPad .. n_distances - 1 + kPad, each taken from the nearest end of the map where it lies outside: any pair of a 32 x 32 block
 // that is not all at one end (one_distance) finds its entry without clamping its distance, and the 16 pairs of a lane lie at fixed
 // places from one another. Finite entries are held within +-1.7e38, so that a type's lowest value, a usual mask, stays
 // finite here and a row of such entries alone is still a row of equal scores, as in the formula.
-__device__ __forceinline__ void stage_bias(const AttnRun& A, int g, float* table, int tid, int nt) {
-    const AttnRun& a = A;
-    for (int x = tid; x < A.group * A.table; x += nt) {
-        const int hl = x / A.table, dist = min(max(x - hl * A.table - kPad, 0), a.n_distances - 1);
-        const int b = min(max(a.buckets[dist], 0), a.n_buckets - 1);
-        const int64_t at = (int64_t)(g * A.group + hl) * a.n_buckets + b;
-        float v;
-        if (a.bias_type == GOI_F32) v = static_cast<const float*>(a.bias)[at];
-        else if (a.bias_type == GOI_F16) v = (float)static_cast<const f16*>(a.bias)[at];
-        else v = (float)static_cast<const bf16*>(a.bias)[at];
-        const float y = v * kLog2e;
-        table[x] = fabsf(v) <= 3.4028235e38f ? fminf(fmaxf(y, -1.7e38f), 1.7e38f) : y;
+struct BiasLds {
+    float* table;
+    float* values;    // [group][n_buckets]
+    uint8_t* bucket;  // [n_distances]
+    __device__ __forceinline__ explicit BiasLds(const AttnRun& A, char* p)
+        : table(reinterpret_cast<float*>(p)), values(table + A.group * A.table),
+          bucket(reinterpret_cast<uint8_t*>(values + A.group * A.n_buckets)) {}
+    // From every thread of the block; ends with the block in step.
+    __device__ __forceinline__ void stage(const AttnRun& A, int g, int tid, int nt) const {
+        for (int x = tid; x < A.n_distances; x += nt) bucket[x] = (uint8_t)min(max(A.buckets[x], 0), A.n_buckets - 1);
+        const int64_t first = (int64_t)g * A.group * A.n_buckets;
+        for (int x = tid; x < A.group * A.n_buckets; x += nt) {
+            float v;
+            if (A.bias_type == GOI_F32) v = static_cast<const float*>(A.bias)[first + x];
+            else if (A.bias_type == GOI_F16) v = (float)static_cast<const f16*>(A.bias)[first + x];
+            else v = (float)static_cast<const bf16*>(A.bias)[first + x];
+            const float y = v * kLog2e;
+            values[x] = fabsf(v) <= 3.4028235e38f ? fminf(fmaxf(y, -1.7e38f), 1.7e38f) : y;
+        }
+        __syncthreads();
+        for (int x = tid; x < A.table; x += nt) {
+            const float* const from = values + bucket[min(max(x - kPad, 0), A.n_distances - 1)];
+            for (int hl = 0; hl < A.group; ++hl) table[hl * A.table + x] = from[hl * A.n_buckets];
+        }
+        __syncthreads();
     }
+};
+__host__ __device__ inline size_t bias_lds(const AttnRun& A) {
+    return A.bias ? ((size_t)A.group * (A.table + A.n_buckets) * sizeof(float) + A.n_distances + 15) / 16 * 16 : 0;
+}
+
+inline size_t attention_lds(const AttnRun& A, int waves) {
+    const int dp = attention_dim_tile(A.dim);
+    return (size_t)tile_buffers(waves) * 2 * tile_rows(dp, waves) * dp * 2 + bias_lds(A);
+}
+// and of the pass over rows: each wave's skewed block and sums by distance (policy_attention_dq.hip)
+constexpr int kSkew = 64, kSkewRows = 16;  // words of a row of the skewed block; it is taken in halves
+inline size_t attention_dq_lds(const AttnRun& A, int waves) {
+    return attention_lds(A, waves) + (A.bias ? (size_t)waves * (kSkewRows * kSkew + A.group * A.table) * sizeof(float) : 0);
 }
 
 // The place in a table of n distances of every pair of a 32-key block at key0 with rows at positions pos_lo .. pos_hi, or -1

@@ -116,14 +116,12 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ __attribute__((aligned(16))) RowValues<RT> values[NBUF];
     T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][q, dout][RT][DP]
-    float* const table = reinterpret_cast<float*>(lds + NBUF * 2 * RT * DP * sizeof(T));
+    const BiasLds bl(A, lds + NBUF * 2 * RT * DP * sizeof(T));
+    const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
     const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
-    if (A.bias) {
-        stage_bias(A, g, table, tid, NT);
-        __syncthreads();
-    }
+    if (A.bias) bl.stage(A, g, tid, NT);
     RowStage<T, DP, RT, NT> stage(A, tid);
     const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
     for (int item = (int)((int64_t)block * A.items / A.per_head); item < end; ++item) {
@@ -142,22 +140,33 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
         clear(dv);
         bool careful = false;
 
-        // the next tile of RT rows at or after m0 with a row that sees a key of the block
-        bool awake = false;
+        // the next tile of RT rows at or after m0 with a row that sees a key of the block: 64 tiles at a time, a lane each
+        uint64_t busy = 0, waking = 0;  // from m0 = from on: tiles that have one, and tiles whose rows all see a key
+        int from = 0, upto = 0;
         const auto seek = [&](int m0) {
-            for (; m0 < A.rows; m0 += RT) {
-                bool any = false;
-                awake = true;
-                for (int b = 0; b < RB; ++b) {
-                    const int x = m0 / 32 + b;
-                    if (x >= A.blocks) continue;
-                    any = any || (blocks[x].lo < block1 && blocks[x].hi > block0);
-                    awake = awake && blocks[x].awake;
+            while (m0 < A.rows) {
+                if (m0 >= upto) {
+                    from = m0;
+                    upto = min((int64_t)m0 + 64 * RT, (int64_t)INT_MAX);
+                    bool any = false, all = true;
+#pragma unroll
+                    for (int b = 0; b < RB; ++b) {
+                        const int64_t x = (int64_t)m0 / 32 + lane * RB + b;
+                        if (x < A.blocks) {
+                            any = any || (blocks[x].lo < block1 && blocks[x].hi > block0);
+                            all = all && blocks[x].awake;
+                        }
+                    }
+                    busy = __ballot(any);
+                    waking = __ballot(all);
                 }
-                if (any) break;
+                const uint64_t left = busy >> ((m0 - from) / RT);
+                if (left) return m0 + __builtin_ctzll(left) * RT;
+                m0 = upto;
             }
-            return m0;
+            return A.rows;
         };
+        const auto awake = [&](int m0) { return (waking >> ((m0 - from) / RT) & 1) != 0; };
         RowInfo mine{INFINITY, 0.0f, 0.0f, 0, 0};
         int my_head = 0, my_step = 0;
         const auto load_values = [&](int m0) {
@@ -185,8 +194,14 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
         int m0 = 0;
         if (A.causal) m0 = (int)(min((int64_t)max(block0 - (L - A.q_steps), 0) * A.group, (int64_t)A.rows) / RT * RT);
         m0 = block0 < block1 ? seek(m0) : A.rows;
+        BlockInfo blk[RB], blk_next[RB];  // of this tile's blocks and the next one's
+        const auto load_blocks = [&](int m0) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) blk_next[b] = blocks[min(m0 / 32 + b, A.blocks - 1)];
+        };
         if (m0 < A.rows) {
-            stage.load(A, n, g, info, m0, awake, tid);
+            load_blocks(m0);
+            stage.load(A, n, g, info, m0, awake(m0), tid);
             load_values(m0);
             stage.store(A, tiles, tiles + RT * DP, tid);
             store_values(values[0]);
@@ -194,9 +209,12 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
         __syncthreads();
         int buf = 0;
         while (m0 < A.rows) {
+#pragma unroll
+            for (int b = 0; b < RB; ++b) blk[b] = blk_next[b];
             const int next = seek(m0 + RT);
             if (next < A.rows) {
-                stage.load(A, n, g, info, next, awake, tid);
+                load_blocks(next);
+                stage.load(A, n, g, info, next, awake(next), tid);
                 load_values(next);
             }
             const T* const qt = tiles + buf * 2 * RT * DP;
@@ -204,14 +222,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
             const RowValues<RT>& val = values[buf];
 #pragma unroll
             for (int b = 0; b < RB; ++b) {
-                const int x = m0 / 32 + b;
-                if (x >= A.blocks) continue;
-                const BlockInfo blk = blocks[x];
-                if (blk.lo >= key0 + 32 || blk.hi <= key0) continue;
+                if (m0 / 32 + b >= A.blocks || blk[b].lo >= key0 + 32 || blk[b].hi <= key0) continue;
                 float16_t p = raw_scores<T, DP>(qt, 32 * b, k, lane);
                 float16_t ds = raw_scores<T, DP>(gt, 32 * b, v, lane);
                 const int r0 = 32 * b + 4 * half;  // the lane's rows: r0 + 8 x + 0 .. 3
-                const int a0 = min(max(blk.pos_lo - (key0 + 31), 0), A.n_distances - 1);
+                const int a0 = min(max(blk[b].pos_lo - (key0 + 31), 0), A.n_distances - 1);
                 if (a0 == A.n_distances - 1) {  // every pair is at the map's last distance or past it
 #pragma unroll
                     for (int x4 = 0; x4 < 4; ++x4) {
@@ -221,7 +236,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                     }
                 } else {
                     // (a key far past the rows, without a causal order, finds the near end's entry in the padding)
-                    const float* const t = table - min(key, blk.pos_lo + kPad - 1);
+                    const float* const t = table - min(key, blk[b].pos_lo + kPad - 1);
 #pragma unroll
                     for (int x4 = 0; x4 < 4; ++x4) {
                         const float4_t top = *reinterpret_cast<const float4_t*>(val.top + r0 + 8 * x4);
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                         p[r] *= inv[e];
                     }
                 }
-                if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
+                if (key0 < blk[b].full_lo || key0 + 32 > blk[b].full_hi) {
 #pragma unroll
                     for (int x4 = 0; x4 < 4; ++x4) {
                         const int4_t lo = *reinterpret_cast<const int4_t*>(val.lo + r0 + 8 * x4);

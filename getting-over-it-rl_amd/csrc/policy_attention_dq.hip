@@ -9,6 +9,12 @@
 namespace goi {
 namespace {
 
+// What the wave's lanes wrote to LDS before is what they read after (LDS serves a wave in order; the compiler is told)
+__device__ __forceinline__ void in_step() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // dq of a wave's 32 rows pair by pair
 template <typename T>
 __device__ void careful_dq(const AttnRun& A, int n, int g, int L, int m0, const float* table, const Row& mine, float my_top,
@@ -40,27 +46,34 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int range[2][NW];
     T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][keys, values][KT][DP]
-    float* const table = reinterpret_cast<float*>(lds + NBUF * 2 * KT * DP * sizeof(T));
+    const BiasLds bl(A, lds + NBUF * 2 * KT * DP * sizeof(T));
+    const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
     const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
-    // the bias by distance, each lane's own sums by bucket, and the place of each distance's bucket in them. A bucket's 64 lanes are
-    // kSumPitch words apart from the next's: adding up many buckets over the lanes, at the end, is then free of bank conflicts
-    float* const all = table + A.group * A.table;  // [NW][n_buckets][kSumPitch]
-    float* const sums = all + wave * A.n_buckets * kSumPitch + lane;
-    uint16_t* const bucket = reinterpret_cast<uint16_t*>(all + NW * A.n_buckets * kSumPitch);  // [A.table]
+    // The bias' gradient: each wave adds up its pairs by head and distance, sums [group][A.table], like the table. A near block
+    // goes through `skew`, 16 rows at a time, each row shifted by its position, so that a column holds one distance: a lane adds up
+    // the columns of one distance, a head's rows at a time. (Adding each pair to its sum by LDS atomics took six times as long.)
+    // Far blocks, all pairs at one end of the map, stay in registers: far[0] the near end, far[1] the far end.
+    float* const own = reinterpret_cast<float*>(lds + NBUF * 2 * KT * DP * sizeof(T) + bias_lds(A));
+    float* const skew = own + wave * (kSkewRows * kSkew + A.group * A.table);
+    float* const sums = skew + kSkewRows * kSkew;
+    float far[2] = {0.0f, 0.0f};
     if (A.bias) {
-        stage_bias(A, g, table, tid, NT);
-        for (int x = tid; x < A.table; x += NT)
-            bucket[x] = (uint16_t)(min(max(A.buckets[min(max(x - kPad, 0), A.n_distances - 1)], 0), A.n_buckets - 1) * kSumPitch);
-        for (int b = 0; b < A.n_buckets; ++b) sums[b * kSumPitch] = 0.0f;
+        for (int x = lane; x < A.group * A.table; x += 64) sums[x] = 0.0f;
+        bl.stage(A, g, tid, NT);
     }
-    // a lane's rows are of the same head in all of a block's items (the host gives a block one item where they are not)
+    // a lane's rows are of the same head, and shifted alike, in all of a block's items (the host gives a block one item where
+    // they are not)
     const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    for (int item = (int)((int64_t)block * A.items / A.per_head); item < end; ++item) {
-        const int n = item / A.tiles, tile = A.tiles - 1 - (item - n * A.tiles);
-        const int L = history(A, n), m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
-        Row row = make_row(A, n, L, m);
+    int item = (int)((int64_t)block * A.items / A.per_head);
+    const auto tile_of = [&](int item) { return A.tiles - 1 - item % A.tiles; };
+    Ahead ahead = look_ahead(A, item / A.tiles, (tile_of(item) * NW + wave) * 32 + (lane & 31));
+    for (; item < end; ++item) {
+        const int n = item / A.tiles, tile = tile_of(item);
+        const int L = ahead.length, m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
+        Row row = make_row(A, ahead, m);
+        if (item + 1 < end) ahead = look_ahead(A, (item + 1) / A.tiles, (tile_of(item + 1) * NW + wave) * 32 + (lane & 31));
         const BlockInfo blk = make_block(A, L, m0, row);
         row.pos = min(max(row.pos, blk.pos_lo), blk.pos_hi);  // also where there is no row
         if (lane == 0) {
@@ -68,7 +81,25 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
             range[1][wave] = blk.hi;
             if (m0 < A.rows) A.block_info[(int64_t)(n * A.kv_heads + g) * A.blocks + m0 / 32] = blk;
         }
+        if (NW > 1) __syncthreads();
+        int lo = blk.lo, hi = blk.hi;
+        if constexpr (NW > 1) {
+            lo = INT_MAX;
+            hi = 0;
+            for (int w = 0; w < NW; ++w) {
+                lo = min(lo, range[0][w]);
+                hi = max(hi, range[1][w]);
+            }
+            lo = __builtin_amdgcn_readfirstlane(lo);
+            hi = __builtin_amdgcn_readfirstlane(hi);
+        }
+        KeyStage<T, DP, KT, NT> ks(A.k, n, g, A.dim, tid), vs(A.v, n, g, A.dim, tid);
+        if (lo < hi) {
+            ks.load(lo, hi, tid);
+            vs.load(lo, hi, tid);
+        }
         const float* const bias = A.bias ? table + row.hl * A.table + kPad : nullptr;
+        const int shift = step_of(A, m) - step_of(A, m0);
         const int head = g * A.group + row.hl;
         half8<T> q[DP / 16], go[DP / 16];
         load_operand<T, DP>(q, A.q.at<T>(n, row.i, head), row.valid, A.dim, lane);
@@ -92,22 +123,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
             if (row.valid && half == 0)
                 A.row_info[(int64_t)(n * A.kv_heads + g) * A.rows + m] = RowInfo{top, inv, delta, row.lo, row.hi};
         }
-        __syncthreads();
-        int lo = INT_MAX, hi = 0;
-        for (int w = 0; w < NW; ++w) {
-            lo = min(lo, range[0][w]);
-            hi = max(hi, range[1][w]);
-        }
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        hi = __builtin_amdgcn_readfirstlane(hi);
 
         float16_t dq[DP / 32];
         clear(dq);
         bool careful = false;
         if (lo < hi) {
-            KeyStage<T, DP, KT, NT> ks(A.k, n, g, A.dim, tid), vs(A.v, n, g, A.dim, tid);
-            ks.load(lo, hi, tid);
-            vs.load(lo, hi, tid);
             ks.store(tiles, lo, hi, tid);
             vs.store(tiles + KT * DP, lo, hi, tid);
             __syncthreads();
@@ -138,20 +158,39 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                         careful = careful || !finite_rows<T, DP>(kt, 32 * b, lane);
                     }
                     if (bias) {
-                        // the lane's own sums, one word a bucket: no two lanes share one, so the order of additions is the
-                        // program's
                         const int one = one_distance(key0, blk.pos_lo, blk.pos_hi, A.n_distances);
                         if (one >= 0) {
                             float t = 0.0f;
 #pragma unroll
                             for (int r = 0; r < 16; ++r) t += s[r];
-                            __hip_atomic_fetch_add(sums + bucket[kPad + one], t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                            if (one > 0) far[1] += t;
+                            else far[0] += t;
                         } else {
-                            const uint16_t* const to = bucket + (kPad + row.pos - key0 - 4 * half - 27);
+                            // column x of the skewed block is distance pos_lo - key0 + 31 - x
+                            float* const sum = sums + kPad + blk.pos_lo - key0 + 31 - lane;
+                            float* const to = skew + (lane & 15) * kSkew + 31 - shift + 4 * half;
 #pragma unroll
-                            for (int r = 0; r < 16; ++r)
-                                __hip_atomic_fetch_add(sums + to[27 - mfma_row(r, 0)], s[r], __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_WORKGROUP);
+                            for (int rows = 0; rows < 32; rows += kSkewRows) {
+#pragma unroll
+                                for (int x = 0; x < kSkewRows * kSkew / 256; ++x)
+                                    reinterpret_cast<float4_t*>(skew)[x * 64 + lane] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                                in_step();
+                                if ((lane & 16) == rows) {
+#pragma unroll
+                                    for (int r = 0; r < 16; ++r) to[mfma_row(r, 0)] = s[r];
+                                }
+                                in_step();
+                                const int turn = (m0 + rows) % A.group;
+                                for (int hl = 0; hl < A.group; ++hl) {
+                                    int r = hl - turn;
+                                    r += r < 0 ? A.group : 0;
+                                    float t = 0.0f;
+#pragma unroll 4
+                                    for (; r < kSkewRows; r += A.group) t += skew[r * kSkew + lane];
+                                    sum[hl * A.table] += t;
+                                }
+                                in_step();
+                            }
                         }
                     }
 #pragma unroll
@@ -176,17 +215,48 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
         __syncthreads();  // the next item overwrites what this one read
     }
     if (A.bias) {
-        // the block's sums: of the lanes whose row is of head hl, over all waves
-        const int tile = A.tiles - 1 - (int)((int64_t)block * A.items / A.per_head) % A.tiles;
-        float* const part = A.part_bias + (int64_t)block * A.heads * A.n_buckets + g * A.group * A.n_buckets;
-        for (int x = tid; x < A.group * A.n_buckets; x += NT) {
-            const int hl = x / A.n_buckets, b = x - hl * A.n_buckets;
-            float t = 0.0f;
-            for (int w = 0; w < NW; ++w) {
-                const int first = (hl - (tile * NW + w) * 32 % A.group + A.group) % A.group;
-                const float* const own = all + (w * A.n_buckets + b) * kSumPitch;
-                for (int l = first; l < 32; l += A.group) t += own[l] + own[l + 32];
+        // the rows' far sums to the ends of their heads (an end's entries in the padding are the end's too)
+        const int m0 = (A.tiles - 1 - (int)((int64_t)block * A.items / A.per_head) % A.tiles) * NW * 32 + wave * 32;
+        skew[lane] = half_sum(far[0]);
+        skew[64 + lane] = half_sum(far[1]);
+        in_step();
+        for (int hl = lane; hl < A.group; hl += 64) {
+            int r = (hl - m0 % A.group + A.group) % A.group;
+            float near_end = 0.0f, far_end = 0.0f;
+            for (; r < 32; r += A.group) {
+                near_end += skew[r];
+                far_end += skew[64 + r];
             }
+            sums[hl * A.table] += near_end;
+            sums[hl * A.table + kPad + A.n_distances - 1] += far_end;
+        }
+        __syncthreads();
+        // the waves' sums by distance in the first one's, then by bucket
+        const int pitch = kSkewRows * kSkew + A.group * A.table;
+        float* const all = own + kSkewRows * kSkew;
+        for (int x = tid; x < A.group * A.table; x += NT) {
+            float t = all[x];
+            for (int w = 1; w < NW; ++w) t += all[w * pitch + x];
+            all[x] = t;
+        }
+        __syncthreads();
+        // each sum by several threads, a range of distances each, where there are threads to spare
+        float* const part = A.part_bias + (int64_t)block * A.heads * A.n_buckets + g * A.group * A.n_buckets;
+        const int outs = A.group * A.n_buckets, parts = max(1, NT / outs);
+        const int ends = A.causal ? min(A.table, kPad + A.k_steps) : A.table;  // no causal pair is further apart
+        for (int x = tid; x < outs * parts; x += NT) {
+            const int at = x % outs, p = x / outs, head = at / A.n_buckets, b = at - head * A.n_buckets;
+            float t = 0.0f;
+            for (int d = ends * p / parts; d < ends * (p + 1) / parts; ++d)
+                if (bl.bucket[min(max(d - kPad, 0), A.n_distances - 1)] == b) t += all[head * A.table + d];
+            if (parts == 1) part[at] = t;
+            else own[x] = t;  // outs * parts <= NT words, over the first wave's skewed block
+        }
+        if (parts == 1) return;
+        __syncthreads();
+        for (int x = tid; x < outs; x += NT) {
+            float t = own[x];
+            for (int p = 1; p < parts; ++p) t += own[p * outs + x];
             part[x] = t;
         }
     }
