@@ -212,37 +212,40 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     }
 }
 
-// Joins the splits of each row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, M the largest m_s. A wave a row.
+// Joins the splits of each row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, M the largest m_s. A block a row, its
+// waves a quarter of the splits each.
 template <typename T>
 __global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
-    const int64_t rows = (int64_t)A.n_worlds * A.kv_heads * A.rows;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
+    __shared__ float4_t shared[4][64];
+    const int64_t rows = (int64_t)A.n_worlds * A.kv_heads * A.rows, row = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float top = -INFINITY;
     for (int s = lane; s < A.splits; s += 64) top = fmaxf(top, A.part_ml[s * rows + row].x);
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, x = 0.0f, y = 0.0f;
-    const bool in = 2 * lane < A.dim;
-    for (int s = 0; s < A.splits; ++s) {
+    float4_t t = {0.0f, 0.0f, 0.0f, 0.0f};  // two elements of the output, and the sum
+    const int d = min(2 * lane, A.dim - 2);
+#pragma unroll 8
+    for (int s = wave; s < A.splits; s += 4) {
         const float2 ml = A.part_ml[s * rows + row];
+        const float2 o = *reinterpret_cast<const float2*>(A.part_o + (s * rows + row) * A.dim + d);
         const float f = exp2_fast(ml.x - base);
-        sum += f * ml.y;
-        if (in) {
-            const float2 o = *reinterpret_cast<const float2*>(A.part_o + (s * rows + row) * A.dim + 2 * lane);
-            x += f * o.x;
-            y += f * o.y;
-        }
+        t[0] += f * o.x;
+        t[1] += f * o.y;
+        t[2] += f * ml.y;
     }
+    shared[wave][lane] = t;
+    __syncthreads();
+    if (wave) return;
+    t = (shared[0][lane] + shared[1][lane]) + (shared[2][lane] + shared[3][lane]);
     const int64_t pair = row / A.rows;
     const int m = (int)(row - pair * A.rows), i = step_of(A, m);
     const int n = (int)(pair / A.kv_heads), head = (int)(pair - (int64_t)n * A.kv_heads) * A.group + m - i * A.group;
-    const float f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+    const float sum = t[2], f = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
     T* const to = A.out.at<T>(n, i, head);
-    if (in) {
-        to[2 * lane] = (T)(x * f);
-        to[2 * lane + 1] = (T)(y * f);
+    if (2 * lane < A.dim) {
+        to[2 * lane] = (T)(t[0] * f);
+        to[2 * lane + 1] = (T)(t[1] * f);
     }
     if (A.stats && lane == 0) A.stats[((int64_t)n * A.heads + head) * A.q_steps + i] = make_float2(top, sum);
 }
@@ -411,7 +414,7 @@ hipError_t launch_forward(const AttnRun& A, hipStream_t st) {
                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL((k_attention<T, DP, NW, true>), grid, block, lds, st, A);
         const int64_t rows = (int64_t)A.n_worlds * A.kv_heads * A.rows;
-        hipLaunchKernelGGL(k_attention_join<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, A);
+        hipLaunchKernelGGL(k_attention_join<T>, dim3((unsigned)rows), dim3(256), 0, st, A);
     } else {
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention<T, DP, NW, false>),
                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -16,13 +16,11 @@ __device__ __forceinline__ int16v mfma(int4_t a, int4_t b, int16v c) {
 // 16 bytes of a row from k on, zeros past width
 __device__ __forceinline__ int4_t row_bytes(const int8_t* row, int k, int width) {
     if (k + 16 <= width) return *reinterpret_cast<const int4_t*>(row + k);
-    union {
-        int4_t v;
-        int8_t b[16];
-    } u;
-    u.v = int4_t{0, 0, 0, 0};
-    for (int e = 0; k + e < width; ++e) u.b[e] = row[k + e];
-    return u.v;
+    int4_t v = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (k + e < width) v[e / 4] |= (int)(uint8_t)row[k + e] << (8 * (e % 4));
+    return v;
 }
 
 __device__ __forceinline__ float bias_at(const GoiInt8& a, int n) {
@@ -44,14 +42,31 @@ __global__ void __launch_bounds__(256) k_int8_few(const GoiInt8 a) {
     int4_t c[MB];
 #pragma unroll
     for (int b = 0; b < MB; ++b) c[b] = int4_t{0, 0, 0, 0};
-#pragma unroll 4
-    for (int k = wave * 64 + 16 * (lane >> 4); k - 16 * (lane >> 4) < a.width; k += 256) {
-        const int4_t x = row_bytes(w, k, a.width);
+    const int8_t* x[MB];
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const int m = min(m0 + 16 * b + (lane & 15), a.rows - 1);
-            c[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, row_bytes(a.x + (int64_t)m * a.x_stride, k, a.width), c[b], 0, 0, 0);
-        }
+    for (int b = 0; b < MB; ++b) x[b] = a.x + (int64_t)min(m0 + 16 * b + (lane & 15), a.rows - 1) * a.x_stride;
+    const int sub = 16 * (lane >> 4), whole = a.width / 256 * 256;
+#pragma unroll 4
+    for (int k = wave * 64 + sub; k < whole; k += 256) {
+        const int4_t f = *reinterpret_cast<const int4_t*>(w + k);
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+            c[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, *reinterpret_cast<const int4_t*>(x[b] + k), c[b], 0, 0, 0);
+    }
+    if (whole + wave * 64 < a.width) {  // the last steps, a wave each
+        const int k = whole + wave * 64 + sub;
+        const int4_t f = row_bytes(w, k, a.width);
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+            c[b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, row_bytes(x[b], k, a.width), c[b], 0, 0, 0);
+    }
+    // what the end needs, while the sums are on their way
+    const int at = n0 + 4 * (lane >> 4);
+    float ws[4], bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        ws[e] = a.w_scales[min(at + e, a.channels - 1)];
+        bias[e] = bias_at(a, min(at + e, a.channels - 1));
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) shared[wave][b][lane] = c[b];
@@ -59,109 +74,159 @@ __global__ void __launch_bounds__(256) k_int8_few(const GoiInt8 a) {
     // wave w finishes row block w: lane l has row l & 15 and channels 4 (l >> 4) .. + 3
     for (int b = wave; b < MB; b += 4) {
         const int4_t s = (shared[0][b][lane] + shared[1][b][lane]) + (shared[2][b][lane] + shared[3][b][lane]);
-        const int m = m0 + 16 * b + (lane & 15), at = n0 + 4 * (lane >> 4);
+        const int m = m0 + 16 * b + (lane & 15);
         if (m >= a.rows) continue;
         const float f = a.x_scales[m];
         T* const y = static_cast<T*>(a.y) + (int64_t)m * a.y_stride;
+#pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (at + e < a.channels) y[at + e] = (T)((float)s[e] * f * a.w_scales[at + e] + bias_at(a, at + e));
+            if (at + e < a.channels) y[at + e] = (T)((float)s[e] * f * ws[e] + bias[e]);
     }
 }
 
-// Many rows: tiles of BM rows and BN channels, four waves of half of each, 128 bytes of k a step through two LDS tiles: the next
-// step's loads are in flight while this one is multiplied.
-template <typename T, int BM, int BN>
-__global__ void __launch_bounds__(256) k_int8(const GoiInt8 a, int tiles_n) {
-    constexpr int WM = BM / 2, WN = BN / 2, RM = WM / 32, RN = WN / 32, NX = BM * 8 / 256, NW = BN * 8 / 256;
-    extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][BM + BN][128]
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+constexpr int kStep = 64;  // bytes of k a step
+
+// LDS of two tiles, or of the four waves' parts of the finished one
+template <typename T, int MB, int NB>
+constexpr int lds_tile() {
+    constexpr int a = 2 * 64 * (MB + NB) * kStep, b = (int)(4 * 32 * (32 * NB + 8) * sizeof(T));
+    return a > b ? a : b;
+}
+
+// Many rows: a block takes BM rows and BN channels, each of its four waves 32 MB rows x 32 NB channels of them, kStep bytes of k
+// a step through two LDS tiles. Memory goes straight to LDS, a wave's 1 KB at a time (16 rows): the next step's loads are in
+// flight while this one is multiplied, in no registers. The channels are the first operand, so that a lane's sums are of one row and
+// groups of four channels; the finished tile leaves through LDS in whole 16-byte pieces of rows.
+template <typename T, int MB, int NB>
+__global__ void __launch_bounds__(256, 2) k_int8(const GoiInt8 a, int tiles_n) {
+    constexpr int BM = 64 * MB, BN = 64 * NB, ROWS = BM + BN, PER = ROWS / 64;  // PER: loads of 16 rows a wave and step
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][BM rows of x, BN of w][kStep]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int place = xcd_place(blockIdx.x, gridDim.x);
     const int m0 = place / tiles_n * BM, n0 = place % tiles_n * BN;
-    int4_t xs[NX], ws[NW];
-    const auto load = [&](int k0) {
+    // row r of the tile, chunk c of 16 bytes, lies at chunk_at<32>(r, c); a load's lane is a place, so it fetches the place's chunk
+    const int8_t* from[PER];
 #pragma unroll
-        for (int j = 0; j < NX; ++j) {
-            const int c = tid + j * 256, m = min(m0 + (c >> 3), a.rows - 1);
-            xs[j] = row_bytes(a.x + (int64_t)m * a.x_stride, k0 + 16 * (c & 7), a.width);
-        }
+    for (int j = 0; j < PER; ++j) {
+        const int r = (wave * PER + j) * 16 + (lane >> 2), ch = (lane & 3) ^ (chunk_at<32>(r, 0) & 3);
+        from[j] = (r < BM ? a.x + (int64_t)min(m0 + r, a.rows - 1) * a.x_stride
+                          : a.w + (int64_t)min(n0 + r - BM, a.channels - 1) * a.w_stride) + 16 * ch;
+    }
+    const auto load = [&](int k0, int buf) {
 #pragma unroll
-        for (int j = 0; j < NW; ++j) {
-            const int c = tid + j * 256, n = min(n0 + (c >> 3), a.channels - 1);
-            ws[j] = row_bytes(a.w + (int64_t)n * a.w_stride, k0 + 16 * (c & 7), a.width);
-        }
+        for (int j = 0; j < PER; ++j)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from[j] + k0),
+                                             (__attribute__((address_space(3))) void*)(lds + (buf * ROWS + (wave * PER + j) * 16) * kStep),
+                                             16, 0, 0);
     };
-    const auto store = [&](int buf) {
-        int4_t* const x = reinterpret_cast<int4_t*>(lds + buf * (BM + BN) * 128);
-        int4_t* const w = x + BM * 8;
+    int16v c[MB][NB];
 #pragma unroll
-        for (int j = 0; j < NX; ++j) x[chunk_at<64>((tid + j * 256) >> 3, tid & 7)] = xs[j];
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int j = 0; j < NW; ++j) w[chunk_at<64>((tid + j * 256) >> 3, tid & 7)] = ws[j];
-    };
-    int16v c[RM][RN];
-#pragma unroll
-    for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < RN; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) c[i][j][r] = 0;
-    load(0);
-    store(0);
-    __syncthreads();
-    int buf = 0;
-    for (int k0 = 0; k0 < a.width; k0 += 128) {
-        const bool more = k0 + 128 < a.width;
-        if (more) load(k0 + 128);
-        const int4_t* const x = reinterpret_cast<const int4_t*>(lds + buf * (BM + BN) * 128);
-        const int4_t* const w = x + BM * 8;
+    const int mw = (wave >> 1) * 32 * MB, nw = (wave & 1) * 32 * NB;  // the wave's part of the tile
+    const auto multiply = [&](int buf) {
+        const int4_t* const x = reinterpret_cast<const int4_t*>(lds + buf * ROWS * kStep);
+        const int4_t* const w = x + BM * (kStep / 16);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            int4_t fx[RM], fw[RN];
+        for (int s = 0; s < kStep / 32; ++s) {
+            int4_t fx[MB], fw[NB];
 #pragma unroll
-            for (int i = 0; i < RM; ++i) fx[i] = x[chunk_at<64>((wave >> 1) * WM + 32 * i + (lane & 31), 2 * s + half)];
+            for (int i = 0; i < MB; ++i) fx[i] = x[chunk_at<32>(mw + 32 * i + (lane & 31), 2 * s + half)];
 #pragma unroll
-            for (int j = 0; j < RN; ++j) fw[j] = w[chunk_at<64>((wave & 1) * WN + 32 * j + (lane & 31), 2 * s + half)];
+            for (int j = 0; j < NB; ++j) fw[j] = w[chunk_at<32>(nw + 32 * j + (lane & 31), 2 * s + half)];
 #pragma unroll
-            for (int i = 0; i < RM; ++i)
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
-                for (int j = 0; j < RN; ++j) c[i][j] = mfma(fx[i], fw[j], c[i][j]);
+                for (int j = 0; j < NB; ++j) c[i][j] = mfma(fw[j], fx[i], c[i][j]);
         }
-        buf ^= 1;
-        if (more) store(buf);
+    };
+    // what is left over of k first, byte by byte at the row's end, so that the steps that follow are whole
+    const int rest = a.width % kStep;
+    if (rest) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = (wave * PER + j) * 16 + (lane >> 2), ch = (lane & 3) ^ (chunk_at<32>(r, 0) & 3);
+            reinterpret_cast<int4_t*>(lds)[r * (kStep / 16) + (lane & 3)] =
+                row_bytes(from[j] - 16 * ch + a.width - rest, 16 * ch, rest);
+        }
+        __syncthreads();
+        multiply(0);
         __syncthreads();
     }
+    int buf = 0;
+    if (a.width >= kStep) load(0, 0);
+    __syncthreads();
+    for (int k0 = kStep; k0 <= a.width - rest; k0 += kStep) {
+        if (k0 < a.width - rest) load(k0, buf ^ 1);
+        multiply(buf);
+        buf ^= 1;
+        __syncthreads();
+    }
+    // the channels' scales and biases
+    float* const scale = reinterpret_cast<float*>(lds + lds_tile<T, MB, NB>());
+    float* const bias = scale + BN;
+    for (int x = tid; x < BN; x += 256) {
+        scale[x] = a.w_scales[min(n0 + x, a.channels - 1)];
+        bias[x] = bias_at(a, min(n0 + x, a.channels - 1));
+    }
+    __syncthreads();
+    // 32 rows x 32 NB channels at a time through the wave's own part of LDS
+    constexpr int PITCH = 32 * NB + 8;  // elements: rows 16 bytes apart from a multiple of the banks
+    T* const out = reinterpret_cast<T*>(lds) + wave * 32 * PITCH;
+    const bool whole = n0 + BN <= a.channels && a.y_stride % (16 / sizeof(T)) == 0 && ((uintptr_t)a.y & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < RN; ++j) {
-        const int n = n0 + (wave & 1) * WN + 32 * j + (lane & 31);
-        if (n >= a.channels) continue;
-        const float f = a.w_scales[n], b = bias_at(a, n);
+    for (int i = 0; i < MB; ++i) {
+        const int m = m0 + mw + 32 * i + (lane & 31);
+        const float f = a.x_scales[min(m, a.rows - 1)];
 #pragma unroll
-        for (int i = 0; i < RM; ++i)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m0 + (wave >> 1) * WM + 32 * i + mfma_row(r, half);
-                if (m < a.rows) static_cast<T*>(a.y)[(int64_t)m * a.y_stride + n] = (T)((float)c[i][j][r] * a.x_scales[m] * f + b);
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int at = 32 * j + 8 * r4 + 4 * half;
+                T y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (T)((float)c[i][j][4 * r4 + e] * f * scale[nw + at + e] + bias[nw + at + e]);
+                struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
+                *reinterpret_cast<Four*>(out + (lane & 31) * PITCH + at) = Four{{y[0], y[1], y[2], y[3]}};
             }
+        __syncthreads();
+        constexpr int V = 16 / sizeof(T), LANES = 32 * NB / V;  // a row's pieces
+        for (int x = lane; x < 32 * LANES; x += 64) {
+            const int r = x / LANES, col = x % LANES * V, row = m0 + mw + 32 * i + r;
+            if (row >= a.rows) continue;
+            T* const to = static_cast<T*>(a.y) + (int64_t)row * a.y_stride + n0 + nw + col;
+            const T* const src = out + r * PITCH + col;
+            if (whole) *reinterpret_cast<int4_t*>(to) = *reinterpret_cast<const int4_t*>(src);
+            else
+                for (int e = 0; e < V; ++e)
+                    if (n0 + nw + col + e < a.channels) to[e] = src[e];
+        }
+        __syncthreads();
     }
 }
 
-template <typename T, int BM, int BN>
+template <typename T, int MB, int NB>
 void launch_tiles(const GoiInt8& a, hipStream_t st) {
+    constexpr int BM = 64 * MB, BN = 64 * NB;
     const int tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.channels + BN - 1) / BN;
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_int8<T, BM, BN>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              2 * (BM + BN) * 128);
-    hipLaunchKernelGGL((k_int8<T, BM, BN>), dim3((unsigned)((int64_t)tiles_m * tiles_n)), dim3(256), 2 * (BM + BN) * 128, st, a,
-                       tiles_n);
+    const int lds = lds_tile<T, MB, NB>() + 2 * BN * (int)sizeof(float);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_int8<T, MB, NB>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL((k_int8<T, MB, NB>), dim3((unsigned)((int64_t)tiles_m * tiles_n)), dim3(256), lds, st, a, tiles_n);
 }
 
 template <typename T>
 void launch(const GoiInt8& a, hipStream_t st) {
     const dim3 few((a.channels + 15) / 16, 1);
+    const auto tiles = [&](int m, int n) { return (int64_t)((a.rows + m - 1) / m) * ((a.channels + n - 1) / n); };
     if (a.rows <= 16) hipLaunchKernelGGL((k_int8_few<T, 1>), few, dim3(256), 0, st, a);
     else if (a.rows <= 32) hipLaunchKernelGGL((k_int8_few<T, 2>), few, dim3(256), 0, st, a);
     else if (a.rows <= 64) hipLaunchKernelGGL((k_int8_few<T, 4>), few, dim3(256), 0, st, a);
-    else if ((int64_t)((a.rows + 127) / 128) * ((a.channels + 127) / 128) >= 256) launch_tiles<T, 128, 128>(a, st);
-    else launch_tiles<T, 64, 64>(a, st);
+    else if (tiles(128, 256) >= 512) launch_tiles<T, 2, 4>(a, st);
+    else if (tiles(128, 128) >= 256) launch_tiles<T, 2, 2>(a, st);
+    else launch_tiles<T, 1, 1>(a, st);
 }
 
 }  // namespace

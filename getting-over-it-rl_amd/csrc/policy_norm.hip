@@ -230,16 +230,17 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
     for (int x = threadIdx.x; x < a.width; x += blockDim.x) part[x] = columns[x];
 }
 
-// dweight from the blocks' parts
-__global__ void __launch_bounds__(256) k_column_sum(const float* parts, int count, int width, void* out, int type) {
-    __shared__ float part[16][17];
-    const int sub = threadIdx.x >> 4, col = blockIdx.x * 16 + (threadIdx.x & 15);
+// dweight from the blocks' parts: a block takes 4 columns, its threads 256 rows of parts at a time
+__global__ void __launch_bounds__(1024) k_column_sum(const float* parts, int count, int width, void* out, int type) {
+    __shared__ float part[16][4];
+    const int sub = threadIdx.x >> 2, col = blockIdx.x * 4 + (threadIdx.x & 3);
     float s = 0.0f;
     if (col < width)
-        for (int r = sub; r < count; r += 16) s += parts[(int64_t)r * width + col];
-    part[sub][threadIdx.x & 15] = s;
+        for (int r = sub; r < count; r += 256) s += parts[(int64_t)r * width + col];
+    for (int d = 32; d >= 4; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) < 4) part[threadIdx.x >> 6][threadIdx.x & 3] = s;
     __syncthreads();
-    if (sub || col >= width) return;
+    if (threadIdx.x >= 4 || col >= width) return;
     s = 0.0f;
     for (int r = 0; r < 16; ++r) s += part[r][threadIdx.x];
     if (type == GOI_F32) static_cast<float*>(out)[col] = s;
@@ -390,7 +391,7 @@ int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_
         else if (a->type == GOI_F16) launch_backward<f16>(*a, vec, tpr, blocks, parts, st);
         else launch_backward<bf16>(*a, vec, tpr, blocks, parts, st);
     }
-    hipLaunchKernelGGL(k_column_sum, dim3((a->width + 15) / 16), dim3(256), 0, st, parts, blocks, a->width, a->dweight,
+    hipLaunchKernelGGL(k_column_sum, dim3((a->width + 3) / 4), dim3(1024), 0, st, parts, blocks, a->width, a->dweight,
                        a->weight_type);
     return launch_error(who);
 }
