@@ -5,6 +5,7 @@ getting-over-it-rl_amd/lib/libgoi_b2.so. There is no fallback: `lib()` raises wh
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -109,6 +110,15 @@ class GoiInt8(ctypes.Structure):
                 ("w_stride", ctypes.c_int64), ("w_scales", _P), ("bias", _P), ("y", _P), ("y_stride", ctypes.c_int64)]
 
 
+# The same as one struct.pack each: filling a structure field by field costs more than the call
+ATTENTION_LAYOUT = struct.Struct("=8if3i3Q9q5Q3q2Q3q3Q9qQ")
+NORM_LAYOUT = struct.Struct("=4if4xQqQqQQqQqQqQQ")
+NORM_BACKWARD_LAYOUT = struct.Struct("=4iQqQqQqQQQqQ")
+INT8_LAYOUT = struct.Struct("=5i4xQqQQqQQQq")
+for _s, _c in ((ATTENTION_LAYOUT, GoiAttention), (NORM_LAYOUT, GoiNorm), (NORM_BACKWARD_LAYOUT, GoiNormBackward),
+               (INT8_LAYOUT, GoiInt8)):
+    assert _s.size == ctypes.sizeof(_c), _c
+
 EXPORTS = ("goi_abi_version", "goi_model_create", "goi_model_destroy", "goi_step", "goi_step_n", "goi_step_n_noalloc",
            "goi_collide", "goi_world_manifold", "goi_apply_motor_actions", "goi_sincos", "goi_packed_layout",
            "goi_model_release_rows", "goi_last_launch", "goi_last_error")
@@ -158,14 +168,14 @@ def lib(path=None):
     L.goi_model_release_rows.restype = ctypes.c_int32
     L.goi_last_launch.argtypes = [ctypes.POINTER(GoiLaunchInfo)]
     L.goi_last_launch.restype = ctypes.c_int32
-    att = ctypes.POINTER(GoiAttention)
-    L.goi_attention_workspace.argtypes = [att, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
-    L.goi_attention_forward.argtypes = [att, _P, ctypes.c_uint64, _P]
-    L.goi_attention_backward.argtypes = [att, _P, ctypes.c_uint64, _P]
-    L.goi_rms_norm.argtypes = [ctypes.POINTER(GoiNorm), _P]
+    # the structures as bytes (the layouts above), which ctypes passes by address, or by reference
+    L.goi_attention_workspace.argtypes = [_P, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
+    L.goi_attention_forward.argtypes = [_P, _P, ctypes.c_uint64, _P]
+    L.goi_attention_backward.argtypes = [_P, _P, ctypes.c_uint64, _P]
+    L.goi_rms_norm.argtypes = [_P, _P]
     L.goi_rms_norm_backward_workspace.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
-    L.goi_rms_norm_backward.argtypes = [ctypes.POINTER(GoiNormBackward), _P, ctypes.c_uint64, _P]
-    L.goi_linear_int8.argtypes = [ctypes.POINTER(GoiInt8), _P]
+    L.goi_rms_norm_backward.argtypes = [_P, _P, ctypes.c_uint64, _P]
+    L.goi_linear_int8.argtypes = [_P, _P]
     L.goi_clip_workspace.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
     L.goi_clip_gradients.argtypes = [ctypes.c_int32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, ctypes.c_uint64, _P]
     for name in POLICY_EXPORTS:

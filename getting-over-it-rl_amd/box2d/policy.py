@@ -13,9 +13,9 @@ stream of its tensors' device and waits for nothing. Tensors whose strides the k
 contiguous, rows that are not 16-byte aligned) are copied first. No counterpart in the reference's physics package, which leaves the
 policy to its caller (README.md:22-24).
 """
-import contextlib
 import ctypes
 import math
+from array import array
 
 import torch
 
@@ -29,33 +29,39 @@ def _need(ok, message, *args):
         raise ValueError(message.format(*args))
 
 
-def _on_gpu(*tensors):
+def _on_gpu(first, *rest):
     """The one CUDA device of the tensors that are given."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        _need(torch.is_tensor(t) and t.is_cuda, "the policy operators take CUDA tensors")
-        _need(dev is None or t.device == dev, "tensors on more than one device")
-        dev = t.device
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("the policy operators take CUDA tensors")
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise ValueError("tensors on more than one device")
     return dev
 
 
-def _guard(dev):
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _stream(dev):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+def _run(dev, call, *args):
+    """A C call on dev's current stream, with dev current. (torch's own two queries behind torch.cuda.current_device and
+    current_stream, without the objects that those make: 4 us a call.)"""
+    index = dev.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        code = call(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            code = call(*args, stream)
+    if code:
+        _abi.check(code)
 
 
 def _rows(x):
     """x (worlds, steps, heads, dim) as the attention kernels read it, and its strides of worlds, steps and heads."""
-    if (x.data_ptr() % 16 or x.stride(3) != 1 or any(x.stride(d) % 8 and x.shape[d] > 1 for d in range(3))
-            or any(x.stride(d) >= 1 << 24 and x.shape[d] > 1 for d in (1, 2))):
-        x = x.clone(memory_format=torch.contiguous_format)
-    s = x.stride()
-    return x, _abi._I64x3(*(s[d] if x.shape[d] > 1 else 0 for d in range(3)))
+    n, t, h, d = x.shape
+    a, b, c, one = x.stride()
+    a, b, c = a if n > 1 else 0, b if t > 1 else 0, c if h > 1 else 0
+    if x.data_ptr() & 15 or one != 1 or (a | b | c) & 7 or b >= 1 << 24 or c >= 1 << 24:
+        return x.clone(memory_format=torch.contiguous_format), (t * h * d, h * d, d)
+    return x, (a, b, c)
 
 
 def _ints(x, shape, name):
@@ -66,7 +72,7 @@ def _ints(x, shape, name):
 
 
 def _ptr(x):
-    return None if x is None else x.data_ptr()
+    return 0 if x is None else x.data_ptr()
 
 
 def distance_buckets(count, reach, two_sided=False, device="cuda"):
@@ -88,56 +94,58 @@ def distance_buckets(count, reach, two_sided=False, device="cuda"):
 
 
 def _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale):
-    """(GoiAttention, device, tensors to keep): the checked inputs of both directions."""
+    """(values of GoiAttention up to out, device, tensors to keep): the checked inputs of both directions."""
     dev = _on_gpu(q, k, v, bias, buckets, first, lengths)
     _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k and v are (worlds, steps, heads, dim)")
     n, tq, h, d = q.shape
-    tk, g = k.shape[1], k.shape[2]
+    _, tk, g, _ = k.shape
+    kind = q.dtype
     _need(tuple(k.shape) == (n, tk, g, d) and k.shape == v.shape, "k and v must be ({}, steps, heads, {}) alike", n, d)
-    _need(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype,
+    _need((kind is torch.bfloat16 or kind is torch.float16) and k.dtype is kind and v.dtype is kind,
           "q, k and v must all be bfloat16 or all float16")
-    a = _abi.GoiAttention()
-    a.n_worlds, a.q_steps, a.k_steps, a.heads, a.kv_heads, a.dim = n, tq, tk, h, g, d
-    a.type, a.causal = _TYPES[q.dtype], int(bool(causal))
-    a.scale = d ** -0.5 if scale is None else float(scale)
-    q, a.q_strides = _rows(q)
-    k, a.k_strides = _rows(k)
-    v, a.v_strides = _rows(v)
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    n_buckets = n_distances = bias_type = 0
     if bias is not None:
         _need(buckets is not None, "a bias needs the buckets of the distances")
-        _need(bias.dim() == 2 and bias.shape[0] == h and bias.dtype in (q.dtype, torch.float32),
+        _need(bias.dim() == 2 and bias.shape[0] == h and bias.dtype in (kind, torch.float32),
               "the bias is (heads, buckets), of q's type or float32")
         _need(buckets.dim() == 1 and buckets.dtype == torch.int32, "buckets must be one row of int32")
         bias, buckets = bias.contiguous(), buckets.contiguous()
-        a.bias, a.buckets, a.bias_type = bias.data_ptr(), buckets.data_ptr(), _TYPES[bias.dtype]
-        a.n_buckets, a.n_distances = bias.shape[1], buckets.shape[0]
+        n_buckets, n_distances, bias_type = bias.shape[1], buckets.shape[0], _TYPES[bias.dtype]
     first = _ints(first, (n, tq), "first")
     lengths = _ints(lengths, (n,), "lengths")
-    a.first, a.lengths = _ptr(first), _ptr(lengths)
-    return a, dev, (q, k, v, bias, buckets, first, lengths)
+    q, qs = _rows(q)
+    k, ks = _rows(k)
+    v, vs = _rows(v)
+    values = (n, tq, tk, h, g, d, _TYPES[kind], 1 if causal else 0, d ** -0.5 if scale is None else scale, n_buckets, n_distances,
+              bias_type, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, _ptr(bias),
+              _ptr(buckets) if bias is not None else 0, _ptr(first), _ptr(lengths))
+    return values, dev, (q, k, v, bias, buckets, first, lengths)
 
 
-def _attention_call(a, dev, backward):
+def _attention_call(values, dev, backward):
     L = _abi.lib()
+    a = _abi.ATTENTION_LAYOUT.pack(*values)
     size = ctypes.c_uint64()
-    _abi.check(L.goi_attention_workspace(ctypes.byref(a), backward, ctypes.byref(size)), L)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-    call = L.goi_attention_backward if backward else L.goi_attention_forward
-    with _guard(dev):
-        _abi.check(call(ctypes.byref(a), _ptr(ws), size.value, _stream(dev)), L)
+    code = L.goi_attention_workspace(a, backward, size)
+    if code:
+        _abi.check(code)
+    size = size.value
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _run(dev, L.goi_attention_backward if backward else L.goi_attention_forward, a, _ptr(ws), size)
+
+
+_NO_GRADIENTS = (0,) * 17  # GoiAttention from dout on
 
 
 def attention_forward(q, k, v, bias=None, buckets=None, first=None, lengths=None, causal=True, scale=None, need_stats=True):
     """(out, stats) of `attention`, without a graph. stats (worlds, heads, steps, 2) float32 is what attention_backward needs
     (None with need_stats=False): each query's largest score times log2(e), and the sum of the powers of two of the scores
     relative to it; minus infinity and 0 where it sees no key."""
-    a, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    out, a.out_strides = _rows(out)
-    stats = torch.empty((q.shape[0], q.shape[2], q.shape[1], 2), dtype=torch.float32, device=dev) if need_stats else None
-    a.out, a.stats = out.data_ptr(), _ptr(stats)
-    _attention_call(a, dev, 0)
+    values, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
+    n, t, h, _ = q.shape
+    out, strides = _rows(torch.empty(q.shape, dtype=q.dtype, device=dev))
+    stats = torch.empty((n, h, t, 2), dtype=torch.float32, device=dev) if need_stats else None
+    _attention_call((*values, out.data_ptr(), *strides, _ptr(stats), *_NO_GRADIENTS), dev, 0)
     del keep
     return out, stats
 
@@ -145,21 +153,19 @@ def attention_forward(q, k, v, bias=None, buckets=None, first=None, lengths=None
 def attention_backward(dout, q, k, v, out, stats, bias=None, buckets=None, first=None, lengths=None, causal=True, scale=None):
     """(dq, dk, dv, dbias) of `attention` for the gradient dout of its output; out and stats are attention_forward's. dbias is
     None without a bias. Every sum has a fixed order: the same inputs give the same bits."""
-    a, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
+    values, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
     _on_gpu(q, dout, out, stats)
     _need(dout.shape == q.shape and out.shape == q.shape and dout.dtype == q.dtype and out.dtype == q.dtype,
           "dout and out must be like q")
-    _need(stats.dtype == torch.float32 and tuple(stats.shape) == (q.shape[0], q.shape[2], q.shape[1], 2),
-          "stats must be float32 (worlds, heads, steps, 2)")
-    dout, a.dout_strides = _rows(dout)
-    out, a.out_strides = _rows(out)
+    n, t, h, _ = q.shape
+    _need(stats.dtype == torch.float32 and tuple(stats.shape) == (n, h, t, 2), "stats must be float32 (worlds, heads, steps, 2)")
+    dout, dout_strides = _rows(dout)
+    out, out_strides = _rows(out)
     stats = stats.contiguous()
-    a.dout, a.out, a.stats = dout.data_ptr(), out.data_ptr(), stats.data_ptr()
-    grads = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v)]
+    (dq, dqs), (dk, dks), (dv, dvs) = (_rows(torch.empty(x.shape, dtype=x.dtype, device=dev)) for x in (q, k, v))
     dbias = None if bias is None else torch.empty(bias.shape, dtype=bias.dtype, device=dev)
-    (dq, a.dq_strides), (dk, a.dk_strides), (dv, a.dv_strides) = map(_rows, grads)
-    a.dq, a.dk, a.dv, a.dbias = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dbias)
-    _attention_call(a, dev, 1)
+    _attention_call((*values, out.data_ptr(), *out_strides, stats.data_ptr(), dout.data_ptr(), *dout_strides, dq.data_ptr(),
+                     dk.data_ptr(), dv.data_ptr(), *dqs, *dks, *dvs, _ptr(dbias)), dev, 1)
     del keep
     return dq, dk, dv, dbias
 
@@ -215,33 +221,30 @@ def _norm_args(x, weight, residual):
     return dev, weight.contiguous()
 
 
-def _norm_call(x, weight, residual, eps, a, want_inv):
-    """Fills and runs GoiNorm (a holds y or values); returns (r, inv)."""
-    rows, width = x.shape[:-1].numel(), x.shape[-1]
-    a.rows, a.width, a.type, a.weight_type, a.eps = rows, width, _TYPES[x.dtype], _TYPES[weight.dtype], eps
+def _norm_call(dev, x, weight, residual, eps, y, y_stride, values, values_stride, scales, want_inv):
+    """Runs GoiNorm (y or values is 0); returns (r, inv)."""
+    shape = x.shape
+    width = shape[-1]
     x2 = _flat(x)
-    a.x, a.x_stride, a.weight = x2.data_ptr(), x2.stride(0), weight.data_ptr()
-    r = x
+    r, inv, res, res_stride = x, None, None, 0
     if residual is not None:
         res = _flat(residual)
-        r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        a.residual, a.residual_stride, a.r, a.r_stride = res.data_ptr(), res.stride(0), r.data_ptr(), width
-    inv = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if want_inv else None
-    a.inv = _ptr(inv)
-    L = _abi.lib()
-    with _guard(x.device):
-        _abi.check(L.goi_rms_norm(ctypes.byref(a), _stream(x.device)), L)
+        res_stride = res.stride(0)
+        r = torch.empty(shape, dtype=x.dtype, device=dev)
+    if want_inv:
+        inv = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+    _run(dev, _abi.lib().goi_rms_norm, _abi.NORM_LAYOUT.pack(
+        x2.shape[0], width, _TYPES[x.dtype], _TYPES[weight.dtype], eps, x2.data_ptr(), x2.stride(0), _ptr(res), res_stride,
+        weight.data_ptr(), r.data_ptr() if res is not None else 0, width, y, y_stride, values, values_stride, scales, _ptr(inv)))
     return r, inv
 
 
 def rms_norm_forward(x, weight, residual=None, eps=1e-6):
     """(y, r, inv) of `rms_norm`, without a graph: r the residual stream (x itself without a residual), inv (...) float32 the
     rows' 1 / sqrt(mean(r ** 2) + eps). rms_norm_backward needs r and inv."""
-    _, weight = _norm_args(x, weight, residual)
-    a = _abi.GoiNorm()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a.y, a.y_stride = y.data_ptr(), x.shape[-1]
-    r, inv = _norm_call(x, weight, residual, eps, a, True)
+    dev, weight = _norm_args(x, weight, residual)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    r, inv = _norm_call(dev, x, weight, residual, eps, y.data_ptr(), x.shape[-1], 0, 0, 0, True)
     return y, r, inv
 
 
@@ -252,23 +255,19 @@ def rms_norm_backward(dy, r, weight, inv, dresidual=None):
     _on_gpu(r, dy, inv)
     _need(dy.shape == r.shape and dy.dtype == r.dtype, "dy must be like r")
     _need(inv.dtype == torch.float32 and inv.shape == r.shape[:-1], "inv must be rms_norm_forward's")
-    a = _abi.GoiNormBackward()
-    rows, width = r.shape[:-1].numel(), r.shape[-1]
-    a.rows, a.width, a.type, a.weight_type = rows, width, _TYPES[r.dtype], _TYPES[weight.dtype]
     dx = torch.empty(r.shape, dtype=r.dtype, device=dev)
     dweight = torch.empty_like(weight)
     dy2, r2, inv = _flat(dy), _flat(r), inv.contiguous()
-    a.dy, a.dy_stride, a.r, a.r_stride = dy2.data_ptr(), dy2.stride(0), r2.data_ptr(), r2.stride(0)
-    if dresidual is not None:
-        dres = _flat(dresidual)
-        a.dresidual, a.dresidual_stride = dres.data_ptr(), dres.stride(0)
-    a.weight, a.inv, a.dx, a.dx_stride, a.dweight = weight.data_ptr(), inv.data_ptr(), dx.data_ptr(), width, dweight.data_ptr()
+    dres = None if dresidual is None else _flat(dresidual)
+    rows, width = r2.shape
     L = _abi.lib()
     size = ctypes.c_uint64()
-    _abi.check(L.goi_rms_norm_backward_workspace(rows, width, ctypes.byref(size)), L)
+    _abi.check(L.goi_rms_norm_backward_workspace(rows, width, size), L)
     ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-    with _guard(dev):
-        _abi.check(L.goi_rms_norm_backward(ctypes.byref(a), _ptr(ws), size.value, _stream(dev)), L)
+    _run(dev, L.goi_rms_norm_backward, _abi.NORM_BACKWARD_LAYOUT.pack(
+        rows, width, _TYPES[r.dtype], _TYPES[weight.dtype], dy2.data_ptr(), dy2.stride(0), r2.data_ptr(), r2.stride(0),
+        _ptr(dres), 0 if dres is None else dres.stride(0), weight.data_ptr(), inv.data_ptr(), dx.data_ptr(), width,
+        dweight.data_ptr()), ws.data_ptr(), size.value)
     return dx, dweight
 
 
@@ -309,13 +308,11 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     each row at 127, and the residual stream r (x itself without a residual). The input of `linear_int8`; rounded once,
     from float32. A row with a value that is not finite has a scale of NaN. No gradient: for acting."""
     dev, weight = _norm_args(x, weight, residual)
-    a = _abi.GoiNorm()
     width = x.shape[-1]
     pitch = (width + 15) // 16 * 16  # rows on 16 bytes, as linear_int8 reads them
     values = torch.empty((*x.shape[:-1], pitch), dtype=torch.int8, device=dev)
     scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    a.values, a.values_stride, a.scales = values.data_ptr(), pitch, scales.data_ptr()
-    r, _ = _norm_call(x, weight, residual, eps, a, False)
+    r, _ = _norm_call(dev, x, weight, residual, eps, 0, 0, values.data_ptr(), pitch, scales.data_ptr(), False)
     return (values if pitch == width else values[..., :width]), scales, r
 
 
@@ -352,20 +349,17 @@ def linear_int8(x, x_scales, weight, weight_scales, bias=None, dtype=torch.bfloa
     _need(dtype in _TYPES, "dtype must be float32, float16 or bfloat16")
     _need(bias is None or (bias.dtype in (dtype, torch.float32) and bias.shape == weight.shape[:1]),
           "the bias is one row of dtype or float32")
-    a = _abi.GoiInt8()
-    a.rows, a.channels, a.width, a.type = x.shape[:-1].numel(), weight.shape[0], weight.shape[1], _TYPES[dtype]
-    y = torch.empty((*x.shape[:-1], a.channels), dtype=dtype, device=dev)
-    x2, a.x_stride = _bytes16(x.flatten(0, -2) if x.dim() > 2 else x if x.dim() == 2 else x[None])
-    w2, a.w_stride = _bytes16(weight)
+    channels, width = weight.shape
+    y = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=dev)
+    x2, x_stride = _bytes16(x if x.dim() == 2 else x[None] if x.dim() == 1 else x.flatten(0, -2))
+    w2, w_stride = _bytes16(weight)
     x_scales, weight_scales = x_scales.contiguous(), weight_scales.contiguous()
-    a.x, a.x_scales, a.w, a.w_scales = x2.data_ptr(), x_scales.data_ptr(), w2.data_ptr(), weight_scales.data_ptr()
+    bias_type = 0
     if bias is not None:
-        bias = bias.contiguous()
-        a.bias, a.bias_type = bias.data_ptr(), _TYPES[bias.dtype]
-    a.y, a.y_stride = y.data_ptr(), a.channels
-    L = _abi.lib()
-    with _guard(dev):
-        _abi.check(L.goi_linear_int8(ctypes.byref(a), _stream(dev)), L)
+        bias, bias_type = bias.contiguous(), _TYPES[bias.dtype]
+    _run(dev, _abi.lib().goi_linear_int8, _abi.INT8_LAYOUT.pack(
+        x2.shape[0], channels, width, _TYPES[dtype], bias_type, x2.data_ptr(), x_stride, x_scales.data_ptr(), w2.data_ptr(),
+        w_stride, weight_scales.data_ptr(), _ptr(bias), y.data_ptr(), channels))
     return y
 
 
@@ -381,25 +375,28 @@ def clip_gradients(grads, max_norm, out=None):
     grads = list(grads)
     outs = grads if out is None else list(out)
     _need(len(outs) == len(grads), "as many outputs as gradients")
-    pairs = [(g, o) for g, o in zip(grads, outs) if g is not None]
-    if not pairs:
+    if any(g is None for g in grads):
+        outs = [o for g, o in zip(grads, outs) if g is not None]
+        grads = [g for g in grads if g is not None]
+    if not grads:
         return torch.zeros((), device="cuda")
-    dev = pairs[0][0].device
-    for g, o in pairs:
-        if not (g.is_cuda and g.device == dev and o.device == dev and g.is_contiguous() and o.is_contiguous()
-                and g.dtype in _TYPES and o.dtype in _TYPES and g.shape == o.shape):
-            raise ValueError("gradients and outputs must be contiguous CUDA tensors of one device, float32, float16 or "
-                             "bfloat16, of equal shapes")
-    n = len(pairs)
-    pointers, longs, ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int32 * n
+    n, dev = len(grads), grads[0].device
+
+    def described(tensors):
+        sizes, kinds = list(map(torch.Tensor.numel, tensors)), [_TYPES.get(t.dtype) for t in tensors]
+        if dev.type != "cuda" or any(i != dev.index for i in map(torch.Tensor.get_device, tensors)) or None in kinds \
+                or not all(map(torch.Tensor.is_contiguous, tensors)):
+            raise ValueError("gradients and outputs must be contiguous CUDA tensors of one device, float32, float16 or bfloat16")
+        return array("Q", map(torch.Tensor.data_ptr, tensors)), array("q", sizes), array("i", kinds)
+
+    from_, sizes, types = described(grads)
+    to, out_sizes, out_types = (from_, sizes, types) if out is None else described(outs)
+    _need(sizes == out_sizes, "outputs must be of their gradients' sizes")
     L = _abi.lib()
     size = ctypes.c_uint64()
-    _abi.check(L.goi_clip_workspace(n, ctypes.byref(size)), L)
+    _abi.check(L.goi_clip_workspace(n, size), L)
     ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    with _guard(dev):
-        _abi.check(L.goi_clip_gradients(
-            n, pointers(*[g.data_ptr() for g, _ in pairs]), pointers(*[o.data_ptr() for _, o in pairs]),
-            longs(*[g.numel() for g, _ in pairs]), ints(*[_TYPES[g.dtype] for g, _ in pairs]),
-            ints(*[_TYPES[o.dtype] for _, o in pairs]), max_norm, norm.data_ptr(), ws.data_ptr(), size.value, _stream(dev)), L)
+    _run(dev, L.goi_clip_gradients, n, *(x.buffer_info()[0] for x in (from_, to, sizes, types, out_types)), max_norm,
+         norm.data_ptr(), ws.data_ptr(), size.value)
     return norm

@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -31,6 +32,18 @@ inline int policy_error(int code, const char* fmt, ...) {
 inline int launch_error(const char* who) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? GOI_OK : policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
+}
+
+// Lets a kernel have `lds` bytes of LDS (64 KB are its own without asking): asked for once a kernel, device and larger size
+template <auto kKernel>
+inline void allow_lds(size_t lds) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    if (lds <= 64 * 1024 || hipGetDevice(&dev) != hipSuccess) return;
+    std::atomic<int>& most = allowed[dev & 63];
+    if (most.load(std::memory_order_relaxed) >= (int)lds) return;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess)
+        most.store((int)lds, std::memory_order_relaxed);
 }
 
 using bf16 = __bf16;

@@ -302,8 +302,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
 template <typename T, int DP, int NW>
 hipError_t launch(const AttnRun& A, hipStream_t st) {
     const size_t lds = attention_lds(A, NW);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_attention_dkv<T, DP, NW>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    allow_lds<k_attention_dkv<T, DP, NW>>(lds);
     hipLaunchKernelGGL((k_attention_dkv<T, DP, NW>), dim3((unsigned)(A.kv_heads * A.per_head)), dim3(64 * NW), lds, st, A);
     return hipGetLastError();
 }

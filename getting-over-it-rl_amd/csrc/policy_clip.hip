@@ -10,8 +10,8 @@ namespace goi {
 namespace {
 
 constexpr int kTensors = 112;      // tables of 32 bytes a tensor within the 4 KB of kernel arguments
-constexpr int kSegment = 16384;    // elements of a tensor that a block takes at a time
-constexpr int kBlocks = 1024;      // blocks of a launch, and partial sums it leaves: 4 a CU
+constexpr int kSegment = 4096;     // elements of a tensor that a block takes at a time
+constexpr int kBlocks = 2048;      // blocks of a launch, and partial sums it leaves: 8 a CU
 
 struct Tensors {
     const void* grad[kTensors];
@@ -35,23 +35,26 @@ __device__ __forceinline__ int tensor_of(const Tensors& t, int s) {
 
 template <typename T>
 __device__ __forceinline__ double squares(const T* x, int n) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), U = 4;  // U loads of V elements in flight a thread
     double s = 0.0;
+    int done = 0;
     if (((uintptr_t)x & 15) == 0) {
         const int whole = n / V;
-        for (int i = threadIdx.x; i < whole; i += blockDim.x) {
+        for (int i = threadIdx.x; i < whole; i += U * 256) {
             union {
                 int4_t raw;
                 T e[V];
-            } u;
-            u.raw = reinterpret_cast<const int4_t*>(x)[i];
+            } u[U];
 #pragma unroll
-            for (int k = 0; k < V; ++k) s += (double)(float)u.e[k] * (double)(float)u.e[k];
+            for (int k = 0; k < U; ++k) u[k].raw = i + k * 256 < whole ? reinterpret_cast<const int4_t*>(x)[i + k * 256] : int4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += (double)(float)u[k].e[e] * (double)(float)u[k].e[e];
         }
-        for (int i = whole * V + threadIdx.x; i < n; i += blockDim.x) s += (double)(float)x[i] * (double)(float)x[i];
-    } else {
-        for (int i = threadIdx.x; i < n; i += blockDim.x) s += (double)(float)x[i] * (double)(float)x[i];
+        done = whole * V;
     }
+    for (int i = done + threadIdx.x; i < n; i += 256) s += (double)(float)x[i] * (double)(float)x[i];
     return s;
 }
 
@@ -65,8 +68,10 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {
 __global__ void __launch_bounds__(256) k_square_sums(const Tensors t, double* parts) {
     __shared__ double shared[4];
     double s = 0.0;
-    for (int seg = blockIdx.x; seg < t.segments; seg += gridDim.x) {
-        const int i = tensor_of(t, seg);
+    const int end = (int)((int64_t)(blockIdx.x + 1) * t.segments / gridDim.x);
+    int seg = (int)((int64_t)blockIdx.x * t.segments / gridDim.x);
+    for (int i = tensor_of(t, seg); seg < end; ++seg) {
+        while (i + 1 < t.count && t.first[i + 1] <= seg) ++i;
         const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
         const int n = (int)min((int64_t)kSegment, t.size[i] - at);
         if (t.type[i] == GOI_F32) s += squares(static_cast<const float*>(t.grad[i]) + at, n);
@@ -79,22 +84,29 @@ __global__ void __launch_bounds__(256) k_square_sums(const Tensors t, double* pa
 
 template <typename T, typename U>
 __device__ __forceinline__ void scale(const T* x, U* y, int n, float f) {
-    constexpr int V = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U));
+    constexpr int V = 16 / (sizeof(T) > sizeof(U) ? sizeof(T) : sizeof(U)), K = 4;  // K loads of V elements in flight a thread
     struct __attribute__((aligned(sizeof(T) * V))) In { T e[V]; };
     struct __attribute__((aligned(sizeof(U) * V))) Out { U e[V]; };
     int done = 0;
     if ((((uintptr_t)x & (sizeof(In) - 1)) | ((uintptr_t)y & (sizeof(Out) - 1))) == 0) {
         const int whole = n / V;
-        for (int i = threadIdx.x; i < whole; i += blockDim.x) {
-            const In a = reinterpret_cast<const In*>(x)[i];
-            Out b;
+        for (int i = threadIdx.x; i < whole; i += K * 256) {
+            In a[K];
 #pragma unroll
-            for (int k = 0; k < V; ++k) b.e[k] = (U)((float)a.e[k] * f);
-            reinterpret_cast<Out*>(y)[i] = b;
+            for (int k = 0; k < K; ++k)
+                if (i + k * 256 < whole) a[k] = reinterpret_cast<const In*>(x)[i + k * 256];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (i + k * 256 >= whole) continue;
+                Out b;
+#pragma unroll
+                for (int e = 0; e < V; ++e) b.e[e] = (U)((float)a[k].e[e] * f);
+                reinterpret_cast<Out*>(y)[i + k * 256] = b;
+            }
         }
         done = whole * V;
     }
-    for (int i = done + threadIdx.x; i < n; i += blockDim.x) y[i] = (U)((float)x[i] * f);
+    for (int i = done + threadIdx.x; i < n; i += 256) y[i] = (U)((float)x[i] * f);
 }
 
 template <typename T>
@@ -104,8 +116,8 @@ __device__ __forceinline__ void scale_to(const T* x, void* out, int type, int64_
     else scale(x, static_cast<bf16*>(out) + at, n, f);
 }
 
-// Each block sums the partial sums itself (a few KB from L2) in the same order. The segments run backwards, so that the
-// first ones read are those that the pass before read last and the last-level cache may still hold.
+// Each block sums the partial sums itself (a few KB from L2) in the same order. A block's segments run backwards, from those
+// that the pass before read last.
 __global__ void __launch_bounds__(256) k_clip(const Tensors t, const double* parts, int count, float max_norm, float* norm) {
     __shared__ double shared[4];
     double s = 0.0;
@@ -114,8 +126,10 @@ __global__ void __launch_bounds__(256) k_clip(const Tensors t, const double* par
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
     float f = max_norm / (total + 1e-6f);
     f = f > 1.0f ? 1.0f : f;
-    for (int seg = t.segments - 1 - (int)blockIdx.x; seg >= 0; seg -= gridDim.x) {
-        const int i = tensor_of(t, seg);
+    const int block = gridDim.x - 1 - blockIdx.x, begin = (int)((int64_t)block * t.segments / gridDim.x);
+    int seg = (int)((int64_t)(block + 1) * t.segments / gridDim.x) - 1;
+    for (int i = tensor_of(t, max(seg, 0)); seg >= begin; --seg) {
+        while (i > 0 && t.first[i] > seg) --i;
         if (t.out[i] == t.grad[i] && f == 1.0f) continue;
         const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
         const int n = (int)min((int64_t)kSegment, t.size[i] - at);

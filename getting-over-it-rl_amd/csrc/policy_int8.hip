@@ -213,7 +213,7 @@ void launch_tiles(const GoiInt8& a, hipStream_t st) {
     constexpr int BM = 64 * MB, BN = 64 * NB;
     const int tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.channels + BN - 1) / BN;
     const int lds = lds_tile<T, MB, NB>() + 2 * BN * (int)sizeof(float);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k_int8<T, MB, NB>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    allow_lds<k_int8<T, MB, NB>>(lds);
     hipLaunchKernelGGL((k_int8<T, MB, NB>), dim3((unsigned)((int64_t)tiles_m * tiles_n)), dim3(256), lds, st, a, tiles_n);
 }
 

@@ -68,7 +68,8 @@ __device__ __forceinline__ void load_weight(const void* w, int type, int col, fl
     for (int e = 0; e < VEC; ++e) f[e] = static_cast<const float*>(w)[col + e];
 }
 
-template <typename T, int VEC, int TPR_WAVES, bool kInt8>
+// kEarly: the weight's loads go out with the row's (few rows: latency counts; many: the registers hold more rows in flight)
+template <typename T, int VEC, int TPR_WAVES, bool kInt8, bool kEarly>
 __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_norm(const GoiNorm a, int tpr) {
     __shared__ float shared[16];
     constexpr int N = kPer / VEC;
@@ -77,8 +78,15 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
     const int64_t at = live ? row : 0;
     const T* const x = static_cast<const T*>(a.x) + at * a.x_stride;
     const T* const res = a.residual ? static_cast<const T*>(a.residual) + at * a.residual_stride : nullptr;
-    float f[kPer];
+    float f[kPer], early[kEarly ? kPer : 1];
     float sum = 0.0f;
+    if constexpr (kEarly) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col < a.width) load_weight<T, VEC>(a.weight, a.weight_type, col, early + j * VEC);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const int col = (j * tpr + sub) * VEC;
@@ -108,7 +116,12 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
         float* const c = f + j * VEC;
         if (res && live) store<T, VEC>(static_cast<T*>(a.r) + at * a.r_stride + col, c);
         float w[VEC];
-        load_weight<T, VEC>(a.weight, a.weight_type, col, w);
+        if constexpr (kEarly) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) w[e] = early[j * VEC + e];
+        } else {
+            load_weight<T, VEC>(a.weight, a.weight_type, col, w);
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) c[e] = c[e] * inv * w[e];
         if constexpr (kInt8) {
@@ -153,38 +166,56 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
     extern __shared__ float columns[];  // [width], where several rows share a block
     constexpr int N = kPer / VEC;
     const int per = TPR_WAVES > 1 ? 1 : 256 / tpr, group = TPR_WAVES > 1 ? 0 : threadIdx.x / tpr, sub = threadIdx.x % tpr;
-    float w[kPer], dw[kPer];
+    // the weight and dresidual's loads have registers to wait in, but in blocks of 1024 threads
+    constexpr bool kHold = TPR_WAVES <= 4;
+    float held[kHold ? kPer : 1], dw[kPer];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         const int col = (j * tpr + sub) * VEC;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) w[j * VEC + e] = dw[j * VEC + e] = 0.0f;
-        if (col < a.width) load_weight<T, VEC>(a.weight, a.weight_type, col, w + j * VEC);
+        for (int e = 0; e < VEC; ++e) dw[j * VEC + e] = 0.0f;
+        if constexpr (kHold)
+            if (col < a.width) load_weight<T, VEC>(a.weight, a.weight_type, col, held + j * VEC);
     }
+    const auto weight = [&](int j, int col, float (&w)[VEC]) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) w[e] = held[j * VEC + e];
+        } else {
+            load_weight<T, VEC>(a.weight, a.weight_type, col, w);
+        }
+    };
     for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows; base += (int64_t)gridDim.x * per) {
         const bool live = base + group < a.rows;
         const int64_t row = live ? base + group : 0;
         const T* const dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
         const T* const r = static_cast<const T*>(a.r) + row * a.r_stride;
+        const T* const res = a.dresidual ? static_cast<const T*>(a.dresidual) + row * a.dresidual_stride : nullptr;
         const float inv = a.inv[row];
-        float g[kPer], x[kPer];
-        float sum = 0.0f;
+        // all of the row's loads before the first use; a lane without a row reads row 0 and counts nothing
+        Chunk<T, VEC> g[N], x[N], back[kHold ? N : 1];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int col = (j * tpr + sub) * VEC;
-            float* const gc = g + j * VEC;
-            float* const xc = x + j * VEC;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) gc[e] = xc[e] = 0.0f;
-            if (col < a.width && live) {
-                load<T, VEC>(dy + col, gc);
-                load<T, VEC>(r + col, xc);
+            if (col < a.width) {
+                g[j] = *reinterpret_cast<const Chunk<T, VEC>*>(dy + col);
+                x[j] = *reinterpret_cast<const Chunk<T, VEC>*>(r + col);
+                if (kHold && res) back[j] = *reinterpret_cast<const Chunk<T, VEC>*>(res + col);
             }
+        }
+        float sum = 0.0f;
+        const float scale = live ? inv : 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int col = (j * tpr + sub) * VEC;
+            if (col >= a.width || !live) continue;
+            float w[VEC];
+            weight(j, col, w);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                dw[j * VEC + e] += gc[e] * xc[e] * (live ? inv : 0.0f);
-                gc[e] *= w[j * VEC + e];
-                sum += gc[e] * xc[e];
+                const float d = (float)g[j].e[e], v = (float)x[j].e[e];
+                dw[j * VEC + e] += d * v * scale;
+                sum += d * w[e] * v;
             }
         }
         sum = row_sum<TPR_WAVES>(sum, tpr, shared);
@@ -193,12 +224,20 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
         for (int j = 0; j < N; ++j) {
             const int col = (j * tpr + sub) * VEC;
             if (col >= a.width || !live) continue;
-            float y[VEC];
+            float w[VEC], y[VEC];
+            weight(j, col, w);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) y[e] = 0.0f;
-            if (a.dresidual) load<T, VEC>(static_cast<const T*>(a.dresidual) + row * a.dresidual_stride + col, y);
+            if (res) {
+                if constexpr (kHold) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[e] += inv * (g[j * VEC + e] - x[j * VEC + e] * along);
+                    for (int e = 0; e < VEC; ++e) y[e] = (float)back[j].e[e];
+                } else {
+                    load<T, VEC>(res + col, y);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[e] += inv * ((float)g[j].e[e] * w[e] - (float)x[j].e[e] * along);
             store<T, VEC>(static_cast<T*>(a.dx) + row * a.dx_stride + col, y);
         }
     }
@@ -253,9 +292,12 @@ __global__ void __launch_bounds__(1024) k_column_sum(const float* parts, int cou
 constexpr int kMaxWidth = 1024 * kPer;
 constexpr int kParts = 1024;  // blocks of the backward pass: 4 a CU
 
-int lanes_for(int width) {
+// The fewest lanes that hold a row; where the rows are few, more of them (up to a wave, a chunk each): a row is then sooner
+// done, and more blocks share the rows
+int lanes_for(int rows, int width, int vec) {
     int tpr = 8;
     while (tpr < 1024 && tpr * kPer < width) tpr *= 2;
+    while (tpr < 64 && (int64_t)rows * tpr < 65536 && tpr * vec < width) tpr *= 2;
     return tpr;
 }
 
@@ -278,10 +320,11 @@ int check(int rows, int width, int type, int weight_type, const char* who) {
 
 template <typename T, int VEC, bool kInt8>
 void launch_norm(const GoiNorm& a, int tpr, hipStream_t st) {
-    if (tpr <= 64)
-        hipLaunchKernelGGL((k_rms_norm<T, VEC, 1, kInt8>), dim3((a.rows + 256 / tpr - 1) / (256 / tpr)), dim3(256), 0, st, a, tpr);
-    else
-        hipLaunchKernelGGL((k_rms_norm<T, VEC, 16, kInt8>), dim3(a.rows), dim3(tpr), 0, st, a, tpr);
+    const dim3 blocks(tpr <= 64 ? (a.rows + 256 / tpr - 1) / (256 / tpr) : a.rows);
+    if (tpr > 256) hipLaunchKernelGGL((k_rms_norm<T, VEC, 16, kInt8, false>), blocks, dim3(tpr), 0, st, a, tpr);
+    else if (tpr > 64) hipLaunchKernelGGL((k_rms_norm<T, VEC, 4, kInt8, false>), blocks, dim3(tpr), 0, st, a, tpr);
+    else if (a.rows <= 1024) hipLaunchKernelGGL((k_rms_norm<T, VEC, 1, kInt8, true>), blocks, dim3(256), 0, st, a, tpr);
+    else hipLaunchKernelGGL((k_rms_norm<T, VEC, 1, kInt8, false>), blocks, dim3(256), 0, st, a, tpr);
 }
 template <typename T, int VEC>
 void launch_norm(const GoiNorm& a, int tpr, hipStream_t st) {
@@ -299,10 +342,10 @@ void launch_norm(const GoiNorm& a, int vec, int tpr, hipStream_t st) {
 
 template <typename T, int VEC>
 void launch_backward(const GoiNormBackward& a, int tpr, int blocks, float* parts, hipStream_t st) {
-    if (tpr <= 64)
-        hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 1>), dim3(blocks), dim3(256), a.width * sizeof(float), st, a, tpr, parts);
+    if (tpr > 256) hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 16>), dim3(blocks), dim3(tpr), 0, st, a, tpr, parts);
+    else if (tpr > 64) hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 4>), dim3(blocks), dim3(tpr), 0, st, a, tpr, parts);
     else
-        hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 16>), dim3(blocks), dim3(tpr), 0, st, a, tpr, parts);
+        hipLaunchKernelGGL((k_rms_norm_backward<T, VEC, 1>), dim3(blocks), dim3(256), a.width * sizeof(float), st, a, tpr, parts);
 }
 template <typename T>
 void launch_backward(const GoiNormBackward& a, int vec, int tpr, int blocks, float* parts, hipStream_t st) {
@@ -313,8 +356,9 @@ void launch_backward(const GoiNormBackward& a, int vec, int tpr, int blocks, flo
     else launch_backward<T, 1>(a, tpr, blocks, parts, st);
 }
 
-int backward_blocks(int rows, int width) {
-    const int tpr = lanes_for(width), per = tpr <= 64 ? 256 / tpr : 1;
+// Enough for any vec (narrower chunks make more lanes a row and more blocks)
+int backward_blocks(int rows, int width, int vec = 1) {
+    const int tpr = lanes_for(rows, width, vec), per = tpr <= 64 ? 256 / tpr : 1;
     return (int)std::min<int64_t>(kParts, ((int64_t)rows + per - 1) / per);
 }
 
@@ -349,7 +393,7 @@ int32_t goi_rms_norm(const GoiNorm* a, void* hip_stream) {
     narrow(&vec, a->weight, 0, size);
     narrow(&vec, a->values, a->values_stride, 1);
     const hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const int tpr = lanes_for(a->width);
+    const int tpr = lanes_for(a->rows, a->width, vec);
     if (a->type == GOI_F32) launch_norm<float>(*a, vec, tpr, st);
     else if (a->type == GOI_F16) launch_norm<f16>(*a, vec, tpr, st);
     else launch_norm<bf16>(*a, vec, tpr, st);
@@ -372,7 +416,7 @@ int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_
     if (rc != GOI_OK) return rc;
     if (!a->dweight || !a->weight || (a->rows > 0 && (!a->dy || !a->r || !a->inv || !a->dx)))
         return policy_error(GOI_E_ARG, "%s: null argument", who);
-    const int blocks = backward_blocks(a->rows, a->width);
+    int blocks = backward_blocks(a->rows, a->width);
     const uint64_t bytes = (uint64_t)blocks * a->width * sizeof(float);
     if (bytes > workspace_bytes || (bytes && (!workspace || (uintptr_t)workspace & 15)))
         return policy_error(GOI_E_ARG, "%s: the workspace is null, misaligned or too small", who);
@@ -386,7 +430,8 @@ int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_
         narrow(&vec, a->dresidual, a->dresidual_stride, size);
         narrow(&vec, a->dx, a->dx_stride, size);
         narrow(&vec, a->weight, 0, size);
-        const int tpr = lanes_for(a->width);
+        blocks = backward_blocks(a->rows, a->width, vec);
+        const int tpr = lanes_for(a->rows, a->width, vec);
         if (a->type == GOI_F32) launch_backward<float>(*a, vec, tpr, blocks, parts, st);
         else if (a->type == GOI_F16) launch_backward<f16>(*a, vec, tpr, blocks, parts, st);
         else launch_backward<bf16>(*a, vec, tpr, blocks, parts, st);
