@@ -94,8 +94,8 @@ def distance_buckets(count, reach, two_sided=False, device="cuda"):
 
 
 def _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale):
-    """(values of GoiAttention up to out, device, tensors to keep): the checked inputs of both directions."""
-    dev = _on_gpu(q, k, v, bias, buckets, first, lengths)
+    """(values of GoiAttention up to out, tensors to keep): the checked inputs of both directions."""
+    _on_gpu(q, k, v, bias, buckets, first, lengths)
     _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k and v are (worlds, steps, heads, dim)")
     n, tq, h, d = q.shape
     _, tk, g, _ = k.shape
@@ -119,10 +119,10 @@ def _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale):
     values = (n, tq, tk, h, g, d, _TYPES[kind], 1 if causal else 0, d ** -0.5 if scale is None else scale, n_buckets, n_distances,
               bias_type, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, _ptr(bias),
               _ptr(buckets) if bias is not None else 0, _ptr(first), _ptr(lengths))
-    return values, dev, (q, k, v, bias, buckets, first, lengths)
+    return values, (q, k, v, bias, buckets, first, lengths)
 
 
-def _attention_call(values, dev, backward):
+def _attention_call(values, q, backward):
     L = _abi.lib()
     a = _abi.ATTENTION_LAYOUT.pack(*values)
     size = ctypes.c_uint64()
@@ -130,8 +130,8 @@ def _attention_call(values, dev, backward):
     if code:
         _abi.check(code)
     size = size.value
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _run(dev, L.goi_attention_backward if backward else L.goi_attention_forward, a, _ptr(ws), size)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _run(q.device, L.goi_attention_backward if backward else L.goi_attention_forward, a, _ptr(ws), size)
 
 
 _NO_GRADIENTS = (0,) * 17  # GoiAttention from dout on
@@ -141,11 +141,11 @@ def attention_forward(q, k, v, bias=None, buckets=None, first=None, lengths=None
     """(out, stats) of `attention`, without a graph. stats (worlds, heads, steps, 2) float32 is what attention_backward needs
     (None with need_stats=False): each query's largest score times log2(e), and the sum of the powers of two of the scores
     relative to it; minus infinity and 0 where it sees no key."""
-    values, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
+    values, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
     n, t, h, _ = q.shape
-    out, strides = _rows(torch.empty(q.shape, dtype=q.dtype, device=dev))
-    stats = torch.empty((n, h, t, 2), dtype=torch.float32, device=dev) if need_stats else None
-    _attention_call((*values, out.data_ptr(), *strides, _ptr(stats), *_NO_GRADIENTS), dev, 0)
+    out, strides = _rows(q.new_empty(q.shape))
+    stats = q.new_empty((n, h, t, 2), dtype=torch.float32) if need_stats else None
+    _attention_call((*values, out.data_ptr(), *strides, _ptr(stats), *_NO_GRADIENTS), q, 0)
     del keep
     return out, stats
 
@@ -153,7 +153,7 @@ def attention_forward(q, k, v, bias=None, buckets=None, first=None, lengths=None
 def attention_backward(dout, q, k, v, out, stats, bias=None, buckets=None, first=None, lengths=None, causal=True, scale=None):
     """(dq, dk, dv, dbias) of `attention` for the gradient dout of its output; out and stats are attention_forward's. dbias is
     None without a bias. Every sum has a fixed order: the same inputs give the same bits."""
-    values, dev, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
+    values, keep = _attention_args(q, k, v, bias, buckets, first, lengths, causal, scale)
     _on_gpu(q, dout, out, stats)
     _need(dout.shape == q.shape and out.shape == q.shape and dout.dtype == q.dtype and out.dtype == q.dtype,
           "dout and out must be like q")
@@ -162,10 +162,10 @@ def attention_backward(dout, q, k, v, out, stats, bias=None, buckets=None, first
     dout, dout_strides = _rows(dout)
     out, out_strides = _rows(out)
     stats = stats.contiguous()
-    (dq, dqs), (dk, dks), (dv, dvs) = (_rows(torch.empty(x.shape, dtype=x.dtype, device=dev)) for x in (q, k, v))
-    dbias = None if bias is None else torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+    (dq, dqs), (dk, dks), (dv, dvs) = (_rows(x.new_empty(x.shape)) for x in (q, k, v))
+    dbias = None if bias is None else bias.new_empty(bias.shape)
     _attention_call((*values, out.data_ptr(), *out_strides, stats.data_ptr(), dout.data_ptr(), *dout_strides, dq.data_ptr(),
-                     dk.data_ptr(), dv.data_ptr(), *dqs, *dks, *dvs, _ptr(dbias)), dev, 1)
+                     dk.data_ptr(), dv.data_ptr(), *dqs, *dks, *dvs, _ptr(dbias)), q, 1)
     del keep
     return dq, dk, dv, dbias
 
@@ -230,9 +230,9 @@ def _norm_call(dev, x, weight, residual, eps, y, y_stride, values, values_stride
     if residual is not None:
         res = _flat(residual)
         res_stride = res.stride(0)
-        r = torch.empty(shape, dtype=x.dtype, device=dev)
+        r = x.new_empty(shape)
     if want_inv:
-        inv = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
+        inv = x.new_empty(shape[:-1], dtype=torch.float32)
     _run(dev, _abi.lib().goi_rms_norm, _abi.NORM_LAYOUT.pack(
         x2.shape[0], width, _TYPES[x.dtype], _TYPES[weight.dtype], eps, x2.data_ptr(), x2.stride(0), _ptr(res), res_stride,
         weight.data_ptr(), r.data_ptr() if res is not None else 0, width, y, y_stride, values, values_stride, scales, _ptr(inv)))
@@ -243,7 +243,7 @@ def rms_norm_forward(x, weight, residual=None, eps=1e-6):
     """(y, r, inv) of `rms_norm`, without a graph: r the residual stream (x itself without a residual), inv (...) float32 the
     rows' 1 / sqrt(mean(r ** 2) + eps). rms_norm_backward needs r and inv."""
     dev, weight = _norm_args(x, weight, residual)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = x.new_empty(x.shape)
     r, inv = _norm_call(dev, x, weight, residual, eps, y.data_ptr(), x.shape[-1], 0, 0, 0, True)
     return y, r, inv
 
@@ -255,7 +255,7 @@ def rms_norm_backward(dy, r, weight, inv, dresidual=None):
     _on_gpu(r, dy, inv)
     _need(dy.shape == r.shape and dy.dtype == r.dtype, "dy must be like r")
     _need(inv.dtype == torch.float32 and inv.shape == r.shape[:-1], "inv must be rms_norm_forward's")
-    dx = torch.empty(r.shape, dtype=r.dtype, device=dev)
+    dx = r.new_empty(r.shape)
     dweight = torch.empty_like(weight)
     dy2, r2, inv = _flat(dy), _flat(r), inv.contiguous()
     dres = None if dresidual is None else _flat(dresidual)
@@ -263,7 +263,7 @@ def rms_norm_backward(dy, r, weight, inv, dresidual=None):
     L = _abi.lib()
     size = ctypes.c_uint64()
     _abi.check(L.goi_rms_norm_backward_workspace(rows, width, size), L)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    ws = r.new_empty(size.value, dtype=torch.uint8)
     _run(dev, L.goi_rms_norm_backward, _abi.NORM_BACKWARD_LAYOUT.pack(
         rows, width, _TYPES[r.dtype], _TYPES[weight.dtype], dy2.data_ptr(), dy2.stride(0), r2.data_ptr(), r2.stride(0),
         _ptr(dres), 0 if dres is None else dres.stride(0), weight.data_ptr(), inv.data_ptr(), dx.data_ptr(), width,
@@ -310,8 +310,8 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6):
     dev, weight = _norm_args(x, weight, residual)
     width = x.shape[-1]
     pitch = (width + 15) // 16 * 16  # rows on 16 bytes, as linear_int8 reads them
-    values = torch.empty((*x.shape[:-1], pitch), dtype=torch.int8, device=dev)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    values = x.new_empty((*x.shape[:-1], pitch), dtype=torch.int8)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     r, _ = _norm_call(dev, x, weight, residual, eps, 0, 0, values.data_ptr(), pitch, scales.data_ptr(), False)
     return (values if pitch == width else values[..., :width]), scales, r
 
@@ -350,7 +350,7 @@ def linear_int8(x, x_scales, weight, weight_scales, bias=None, dtype=torch.bfloa
     _need(bias is None or (bias.dtype in (dtype, torch.float32) and bias.shape == weight.shape[:1]),
           "the bias is one row of dtype or float32")
     channels, width = weight.shape
-    y = torch.empty((*x.shape[:-1], channels), dtype=dtype, device=dev)
+    y = x.new_empty((*x.shape[:-1], channels), dtype=dtype)
     x2, x_stride = _bytes16(x if x.dim() == 2 else x[None] if x.dim() == 1 else x.flatten(0, -2))
     w2, w_stride = _bytes16(weight)
     x_scales, weight_scales = x_scales.contiguous(), weight_scales.contiguous()
@@ -395,8 +395,8 @@ def clip_gradients(grads, max_norm, out=None):
     L = _abi.lib()
     size = ctypes.c_uint64()
     _abi.check(L.goi_clip_workspace(n, size), L)
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), device=dev, dtype=torch.float32)
+    ws = grads[0].new_empty(size.value, dtype=torch.uint8)
+    norm = grads[0].new_empty((), dtype=torch.float32)
     _run(dev, L.goi_clip_gradients, n, *(x.buffer_info()[0] for x in (from_, to, sizes, types, out_types)), max_norm,
          norm.data_ptr(), ws.data_ptr(), size.value)
     return norm

@@ -46,6 +46,9 @@ inline void allow_lds(size_t lds) {
         most.store((int)lds, std::memory_order_relaxed);
 }
 
+// out[x] = the sum of parts[.][x] over `count` rows of `width`, in a fixed order, as type (policy_norm.hip)
+void column_sum(const float* parts, int count, int width, void* out, int type, hipStream_t st);
+
 using bf16 = __bf16;
 using f16 = _Float16;
 typedef short short4_t __attribute__((ext_vector_type(4)));

@@ -41,7 +41,7 @@ __device__ void careful_rows(const AttnRun& A, int n, int g, int L, int split, i
 // NW waves of 32 packed rows each share tiles of KT keys. Two tiles of LDS (one for a single wave, which needs no barrier):
 // the next tile's loads are in flight while this one is computed.
 template <typename T, int DP, int NW, bool kSplit>
-__global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_attention(const AttnRun A) {
+__global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 || NW < 4 ? 2 : 3) k_attention(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int range[2][NW];
@@ -51,32 +51,30 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
     const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
-    if (A.bias) bl.stage(A, g, tid, NT);
     // the later row tiles of a causal window see the most keys: they go first
-    const auto place_of = [&](int item, int* split, int* tile) {
-        int n = item / A.tiles;
-        *tile = A.tiles - 1 - (item - n * A.tiles);
-        *split = 0;
-        if (kSplit) {
-            const int x = n / A.splits;
-            *split = n - x * A.splits;
-            n = x;
-        }
-        return n;
-    };
     const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    int item = (int)((int64_t)block * A.items / A.per_head), split, tile;
-    int n = place_of(item, &split, &tile);
-    Ahead ahead = look_ahead(A, n, (tile * NW + wave) * 32 + (lane & 31));
-    for (; item < end; ++item) {
-        n = place_of(item, &split, &tile);
-        const int L = ahead.length, m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
+    int item = (int)((int64_t)block * A.items / A.per_head);
+    int n = item / A.tiles, tile = A.tiles - 1 - (item - n * A.tiles), split = 0;
+    if (kSplit) {
+        const int x = n / A.splits;
+        split = n - x * A.splits;
+        n = x;
+    }
+    const auto row_of = [&](int tile) { return (tile * NW + wave) * 32 + (lane & 31); };
+    Ahead ahead = look_ahead(A, n, row_of(tile));
+    if (A.bias) bl.stage(A, g, tid, NT);
+    int next_n = n, next_tile = tile, next_split = split;
+    for (; item < end; ++item, n = next_n, tile = next_tile, split = next_split) {
+        const int L = ahead.length, m = row_of(tile), m0 = (tile * NW + wave) * 32;
         Row row = make_row(A, ahead, m);
-        if (item + 1 < end) {
-            int s, t;
-            const int next = place_of(item + 1, &s, &t);
-            ahead = look_ahead(A, next, (t * NW + wave) * 32 + (lane & 31));
+        if (--next_tile < 0) {
+            next_tile = A.tiles - 1;
+            if (!kSplit || ++next_split == A.splits) {
+                next_split = 0;
+                ++next_n;
+            }
         }
+        if (item + 1 < end) ahead = look_ahead(A, next_n, row_of(next_tile));
         if (kSplit) {
             row.lo = max(row.lo, split * A.span);
             row.hi = min(row.hi, (split + 1) * A.span);
@@ -114,7 +112,6 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
         float16_t o[DP / 32];
         clear(o);
         float top = -INFINITY, sum = 0.0f;
-        bool careful = false;
         if (lo < hi) {
             KeyStage<T, DP, KT, NT> ks(A.k, n, g, A.dim, tid), vs(A.v, n, g, A.dim, tid);
             ks.load(lo, hi, tid);
@@ -139,14 +136,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                         const int key0 = k0 + 32 * b;
                         s[b] = raw_scores<T, DP>(kt, 32 * b, q, lane);
                         scale_scores(s[b], A.c, bias, A.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
-                        if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                const int key = key0 + mfma_row(r, half);
-                                s[b][r] = key >= row.lo && key < row.hi ? s[b][r] : -INFINITY;
-                            }
-                            careful = careful || !finite_rows<T, DP>(vt, 32 * b, lane);
-                        }
+                        mask_keys(s[b], -INFINITY, row, blk, key0, half);
 #pragma unroll
                         for (int r = 0; r < 16; ++r) best = fmaxf(best, s[b][r]);
                     }
@@ -207,7 +197,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
             store_row<T, DP>(A.out.at<T>(n, row.i, head), o, sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f, A.dim, half);
             if (A.stats && half == 0) A.stats[((int64_t)n * A.heads + head) * A.q_steps + row.i] = make_float2(top, sum);
         }
-        if (careful) careful_rows<T, kSplit>(A, n, g, L, split, m0, table, row, top, sum, lane);
+        if (!all_finite(o)) careful_rows<T, kSplit>(A, n, g, L, split, m0, table, row, top, sum, lane);
         __syncthreads();  // the next item overwrites what this one read
     }
 }
@@ -248,24 +238,6 @@ __global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
         to[2 * lane + 1] = (T)(t[1] * f);
     }
     if (A.stats && lane == 0) A.stats[((int64_t)n * A.heads + head) * A.q_steps + i] = make_float2(top, sum);
-}
-
-// dbias from the blocks' parts [count][columns]: block (x, y) sums rows y, y + gridDim.y, ... of 64 columns, then the
-// second launch (one row of blocks) the sums. Fixed order.
-__global__ void __launch_bounds__(256) k_bias_sum(const float* parts, int count, int columns, float* sums, void* out, int type) {
-    __shared__ float part[4][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), sub = threadIdx.x >> 6;
-    float s = 0.0f;
-    if (col < columns)
-        for (int64_t r = (int64_t)blockIdx.y * 4 + sub; r < count; r += (int64_t)gridDim.y * 4) s += parts[r * columns + col];
-    part[sub][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (sub || col >= columns) return;
-    s = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-    if (sums) sums[(int64_t)blockIdx.y * columns + col] = s;
-    else if (type == GOI_F32) static_cast<float*>(out)[col] = s;
-    else if (type == GOI_F16) static_cast<f16*>(out)[col] = (f16)s;
-    else static_cast<bf16*>(out)[col] = (bf16)s;
 }
 
 // ---------------------------------------------------------------- host
@@ -378,11 +350,10 @@ uint64_t forward_bytes(const AttnRun& A) {
     return round16(rows * sizeof(float2)) + rows * A.dim * sizeof(float);
 }
 
-// The backward scratch: row and block infos, dbias' parts and their first sums.
-constexpr int kBiasSums = 128;
+// The backward scratch: row and block infos, and dbias' parts.
 struct BackwardPlan {
     int waves;
-    uint64_t blocks_at, parts_at, sums_at, bytes;
+    uint64_t blocks_at, parts_at, bytes;
 };
 // Fills in the launch of the pass over rows
 int plan_backward(AttnRun* run, BackwardPlan* plan, const char* who) {
@@ -400,8 +371,7 @@ int plan_backward(AttnRun* run, BackwardPlan* plan, const char* who) {
     p.blocks_at = round16(pairs * A.rows * sizeof(RowInfo));
     p.parts_at = round16(p.blocks_at + pairs * A.blocks * sizeof(BlockInfo));
     const uint64_t columns = a.bias ? (uint64_t)a.heads * a.n_buckets : 0;
-    p.sums_at = round16(p.parts_at + A.per_head * columns * sizeof(float));
-    p.bytes = p.sums_at + kBiasSums * columns * sizeof(float);
+    p.bytes = p.parts_at + A.per_head * columns * sizeof(float);
     return GOI_OK;
 }
 
@@ -513,13 +483,7 @@ int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t 
     if (rows) e = launch_attention_dq(A, p.waves, st);
     if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));
     if (a->bias) {
-        const int columns = a->heads * a->n_buckets, x = (columns + 63) / 64;
-        float* const sums = reinterpret_cast<float*>(ws + p.sums_at);
-        const int count = rows ? A.per_head : 0, y = std::max(1, std::min(kBiasSums, (count + 3) / 4));
-        if (y > 1)
-            hipLaunchKernelGGL(k_bias_sum, dim3(x, y), dim3(256), 0, st, A.part_bias, count, columns, sums, nullptr, 0);
-        hipLaunchKernelGGL(k_bias_sum, dim3(x, 1), dim3(256), 0, st, y > 1 ? sums : A.part_bias, y > 1 ? y : count, columns,
-                           nullptr, a->dbias, a->bias_type);
+        column_sum(A.part_bias, rows ? A.per_head : 0, a->heads * a->n_buckets, a->dbias, a->bias_type, st);
         rc = launch_error(who);
         if (rc != GOI_OK) return rc;
     }

@@ -146,14 +146,15 @@ __device__ __forceinline__ BlockInfo make_block(const AttnRun& A, int L, int m0,
 }
 
 // ROWS rows of a tensor on their way to an LDS tile: load() issues the loads (inside the tensor, whatever the row), store()
-// writes the tile with zeros in the rows from hi on and past dim. A thread's chunks keep their places in every tile, so a
-// whole tile's addresses are the tile's own (the same for every lane) and offsets computed once.
+// writes the tile with zeros in the rows from hi on and past dim. A thread's chunks keep their places in every tile, whole
+// rows apart, so a whole tile's addresses are the tile's own (the same for every lane) and one offset computed once.
 template <typename T, int DP, int ROWS, int NT>
 struct KeyStage {
     static constexpr int N = ROWS * (DP / 8) / NT;
     static_assert(ROWS * (DP / 8) % NT == 0, "whole chunks a thread");
+    static constexpr int kNext = NT / (DP / 8);  // rows from a thread's chunk to its next
     int4_t x[N];
-    uint32_t at[N];
+    uint32_t at;  // of the thread's first chunk in a tile
     const char* base;
     int32_t stride;
     int dim;
@@ -161,21 +162,19 @@ struct KeyStage {
     __device__ __forceinline__ static int chunk_of(int j, int tid) { return (tid + j * NT) % (DP / 8); }
     __device__ __forceinline__ KeyStage(const View& x, int n, int head, int d, int tid)
         : base(x.at<char>(n, 0, head)), stride(x.step), dim(d) {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            at[j] = (uint32_t)row_of(j, tid) * (uint32_t)stride + (chunk_of(j, tid) * 8 < dim ? chunk_of(j, tid) * 16 : 0);
+        at = (uint32_t)row_of(0, tid) * (uint32_t)stride + (chunk_of(0, tid) * 8 < dim ? chunk_of(0, tid) * 16 : 0);
     }
     __device__ __forceinline__ void load(int row0, int hi, int tid) {
         const char* const from = base + (int64_t)row0 * stride;
         if (row0 + ROWS <= hi) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = *reinterpret_cast<const int4_t*>(from + at[j]);
+            for (int j = 0; j < N; ++j) x[j] = *reinterpret_cast<const int4_t*>(from + (int64_t)(j * kNext) * stride + at);
         } else {
             const int last = hi - 1 - row0;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const int over = max(row_of(j, tid) - last, 0);
-                x[j] = *reinterpret_cast<const int4_t*>(from + (at[j] - (uint32_t)over * (uint32_t)stride));
+                x[j] = *reinterpret_cast<const int4_t*>(from + (int64_t)(j * kNext - over) * stride + at);
             }
         }
     }
@@ -305,29 +304,34 @@ __device__ __forceinline__ void store_row(T* row, const float16_t (&o)[DP / 32],
         }
 }
 
-// ---- values that are not finite in blocks that some rows do not see
-//
-// A product takes 0 * NaN as NaN, so in a block where some pair is masked, a row of the tile that is not finite would reach
-// the sums of those that do not see it. Such blocks are looked through (finite_rows); a wave that found one computes its results
-// again at the end, pair by pair, with the pairs that do not count left out (careful_score and the loops that call it).
-
-// Whether all elements of 32 rows of a tile are finite: the largest exponent field among them is not all ones
-template <typename T, int DP>
-__device__ __forceinline__ bool finite_rows(const T* tile, int row0, int lane) {
-    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
-    ushort2_t most = {0, 0};
+// s, with `other` where the lane's row does not see the key: 16 keys from key0 on, the bounds that the block needs only
+__device__ __forceinline__ void mask_keys(float16_t& s, float other, const Row& row, const BlockInfo& blk, int key0, int half) {
+    if (key0 < blk.full_lo) {
+        const int lo = row.lo - key0 - 4 * half;
 #pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {  // 32 rows of DP / 8 chunks, in the order in which they lie
-        union {
-            int4_t v;
-            ushort2_t h[4];
-        } u;
-        u.v = reinterpret_cast<const int4_t*>(tile)[row0 * (DP / 8) + j * 64 + lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, u.h[e] & (unsigned short)0x7fff);
+        for (int r = 0; r < 16; ++r) s[r] = mfma_row(r, 0) < lo ? other : s[r];
     }
-    constexpr unsigned short kInf = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80 : 0x7c00;
-    return !__any(most[0] >= kInf || most[1] >= kInf);
+    if (key0 + 32 > blk.full_hi) {
+        const int hi = row.hi - key0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = mfma_row(r, 0) < hi ? s[r] : other;
+    }
+}
+
+// ---- values that are not finite
+//
+// A product takes 0 * NaN as NaN, so a row of a tile that is not finite reaches the sums of all rows whose blocks hold it, also
+// of those that do not see it. A wave whose results are not all finite therefore computes them again, pair by pair, with the pairs that
+// do not count left out (careful_score and the loops that call it).
+
+template <int N>
+__device__ __forceinline__ bool all_finite(const float16_t (&o)[N]) {
+    float x = 0.0f;
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x += o[b][r] * 0.0f;
+    return !__any(x != 0.0f);  // 0 * infinity and 0 * NaN are NaN
 }
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -345,6 +349,14 @@ __device__ __forceinline__ float2 two_elements(const T* row, int dim, int lane) 
 __device__ __forceinline__ float careful_score(const AttnRun& A, float2 x, float2 y, const float* bias, int distance) {
     const float s = wave_sum(x.x * y.x + x.y * y.y) * A.c;
     return bias ? s + bias[min(max(distance + A.origin, 0), A.n_distances - 1)] : s;
+}
+
+// Says that the sums are in registers here. At the end of a loop whose body may be skipped it keeps the compiler from holding
+// them twice, once for each way.
+template <int N>
+__device__ __forceinline__ void keep_once(float16_t (&o)[N]) {
+#pragma unroll
+    for (int b = 0; b < N; ++b) asm volatile("" : "+a"(o[b]));
 }
 
 template <int N>

@@ -8,33 +8,31 @@ namespace goi {
 namespace {
 
 // A tile of packed rows on its way to LDS. Rows that see no key are stored as zeros: what they hold (the steps after an
-// episode's end, say) must not reach a sum. Where the group divides a tile, the rows of a tile keep their places relative to its
-// first step, as in KeyStage.
+// episode's end, say) must not reach a sum. Where the group divides the rows between a thread's chunks, these keep their
+// places relative to the tile's first step, as in KeyStage.
 template <typename T, int DP, int ROWS, int NT>
 struct RowStage {
     static constexpr int N = ROWS * (DP / 8) / NT;
     int4_t q[N], go[N];
-    uint32_t q_at[N], go_at[N];
+    uint32_t q_at, go_at;        // of the thread's first chunk; the next ones lie whole rows further on
     __device__ __forceinline__ static int row_of(int j, int tid) { return (tid + j * NT) / (DP / 8); }
     __device__ __forceinline__ static int chunk_of(int j, int tid) { return (tid + j * NT) % (DP / 8); }
+    static constexpr int kNext = NT / (DP / 8);  // rows from a thread's chunk to its next
     __device__ __forceinline__ RowStage(const AttnRun& A, int tid) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int i = step_of(A, row_of(j, tid)), hl = row_of(j, tid) - i * A.group;
-            const int d = chunk_of(j, tid) * 8 < A.dim ? chunk_of(j, tid) * 16 : 0;
-            q_at[j] = (uint32_t)(i * A.q.step + hl * A.q.head + d);
-            go_at[j] = (uint32_t)(i * A.dout.step + hl * A.dout.head + d);
-        }
+        const int i = step_of(A, row_of(0, tid)), hl = row_of(0, tid) - i * A.group;
+        const int d = chunk_of(0, tid) * 8 < A.dim ? chunk_of(0, tid) * 16 : 0;
+        q_at = (uint32_t)(i * A.q.step + hl * A.q.head + d);
+        go_at = (uint32_t)(i * A.dout.step + hl * A.dout.head + d);
     }
     __device__ __forceinline__ void load(const AttnRun& A, int n, int g, const RowInfo* info, int m0, bool awake, int tid) {
-        if (m0 + ROWS <= A.rows && ROWS % A.group == 0) {
-            const int i = step_of(A, m0);
+        if (m0 + ROWS <= A.rows && kNext % A.group == 0) {
+            const int i = step_of(A, m0), next = step_of(A, kNext);
             const char* const q0 = A.q.at<char>(n, i, g * A.group);
             const char* const g0 = A.dout.at<char>(n, i, g * A.group);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                q[j] = *reinterpret_cast<const int4_t*>(q0 + q_at[j]);
-                go[j] = *reinterpret_cast<const int4_t*>(g0 + go_at[j]);
+                q[j] = *reinterpret_cast<const int4_t*>(q0 + (int64_t)j * next * A.q.step + q_at);
+                go[j] = *reinterpret_cast<const int4_t*>(g0 + (int64_t)j * next * A.dout.step + go_at);
             }
         } else {
 #pragma unroll
@@ -138,7 +136,6 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
         float16_t dk[DP / 32], dv[DP / 32];
         clear(dk);
         clear(dv);
-        bool careful = false;
 
         // the next tile of RT rows at or after m0 with a row that sees a key of the block: 64 tiles at a time, a lane each
         uint64_t busy = 0, waking = 0;  // from m0 = from on: tiles that have one, and tiles whose rows all see a key
@@ -224,7 +221,9 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
             for (int b = 0; b < RB; ++b) {
                 if (m0 / 32 + b >= A.blocks || blk[b].lo >= key0 + 32 || blk[b].hi <= key0) continue;
                 float16_t p = raw_scores<T, DP>(qt, 32 * b, k, lane);
+                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);  // one product's operands at a time: registers
                 float16_t ds = raw_scores<T, DP>(gt, 32 * b, v, lane);
+                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
                 const int r0 = 32 * b + 4 * half;  // the lane's rows: r0 + 8 x + 0 .. 3
                 const int a0 = min(max(blk[b].pos_lo - (key0 + 31), 0), A.n_distances - 1);
                 if (a0 == A.n_distances - 1) {  // every pair is at the map's last distance or past it
@@ -256,21 +255,29 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                         p[r] *= inv[e];
                     }
                 }
-                if (key0 < blk[b].full_lo || key0 + 32 > blk[b].full_hi) {
+                if (key0 < blk[b].full_lo) {
 #pragma unroll
                     for (int x4 = 0; x4 < 4; ++x4) {
                         const int4_t lo = *reinterpret_cast<const int4_t*>(val.lo + r0 + 8 * x4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            p[4 * x4 + e] = key >= lo[e] ? p[4 * x4 + e] : 0.0f;
+                            ds[4 * x4 + e] = key >= lo[e] ? ds[4 * x4 + e] : 0.0f;
+                        }
+                    }
+                }
+                if (key0 + 32 > blk[b].full_hi) {
+#pragma unroll
+                    for (int x4 = 0; x4 < 4; ++x4) {
                         const int4_t hi = *reinterpret_cast<const int4_t*>(val.hi + r0 + 8 * x4);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * x4 + e;
-                            const bool sees = key >= lo[e] && key < hi[e];
-                            p[r] = sees ? p[r] : 0.0f;
-                            ds[r] = sees ? ds[r] : 0.0f;
+                            p[4 * x4 + e] = key < hi[e] ? p[4 * x4 + e] : 0.0f;
+                            ds[4 * x4 + e] = key < hi[e] ? ds[4 * x4 + e] : 0.0f;
                         }
                     }
-                    careful = careful || !finite_rows<T, DP>(qt, 32 * b, lane) || !finite_rows<T, DP>(gt, 32 * b, lane);
                 }
+                if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x2 = 0; x2 < 2; ++x2) {
                     const half8<T> pf = to_operand<T>(p, x2), sf = to_operand<T>(ds, x2);
@@ -280,6 +287,10 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                         dk[d] = mfma(column_fragment<T, DP>(qt, 32 * b + 16 * x2, 32 * d, lane), sf, dk[d]);
                     }
                 }
+            }
+            if constexpr (DP == 128) {
+                keep_once(dk);
+                keep_once(dv);
             }
             if (NBUF == 1) __syncthreads();
             else buf ^= 1;
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
             store_row<T, DP>(A.dk.at<T>(n, key, g), dk, A.scale, A.dim, half);
             store_row<T, DP>(A.dv.at<T>(n, key, g), dv, 1.0f, A.dim, half);
         }
-        if (careful) careful_keys<T>(A, n, g, L, key0, table, info, lane);
+        if (!(all_finite(dk) && all_finite(dv))) careful_keys<T>(A, n, g, L, key0, table, info, lane);
         __syncthreads();  // the next item overwrites what this one read
     }
 }

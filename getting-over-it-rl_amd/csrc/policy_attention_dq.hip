@@ -59,21 +59,26 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     float* const skew = own + wave * (kSkewRows * kSkew + A.group * A.table);
     float* const sums = skew + kSkewRows * kSkew;
     float far[2] = {0.0f, 0.0f};
-    if (A.bias) {
-        for (int x = lane; x < A.group * A.table; x += 64) sums[x] = 0.0f;
-        bl.stage(A, g, tid, NT);
-    }
     // a lane's rows are of the same head, and shifted alike, in all of a block's items (the host gives a block one item where
     // they are not)
     const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
     int item = (int)((int64_t)block * A.items / A.per_head);
-    const auto tile_of = [&](int item) { return A.tiles - 1 - item % A.tiles; };
-    Ahead ahead = look_ahead(A, item / A.tiles, (tile_of(item) * NW + wave) * 32 + (lane & 31));
-    for (; item < end; ++item) {
-        const int n = item / A.tiles, tile = tile_of(item);
-        const int L = ahead.length, m0 = (tile * NW + wave) * 32, m = m0 + (lane & 31);
+    int n = item / A.tiles, tile = A.tiles - 1 - (item - n * A.tiles);
+    const auto row_of = [&](int tile) { return (tile * NW + wave) * 32 + (lane & 31); };
+    Ahead ahead = look_ahead(A, n, row_of(tile));
+    if (A.bias) {
+        for (int x = lane; x < A.group * A.table; x += 64) sums[x] = 0.0f;
+        bl.stage(A, g, tid, NT);
+    }
+    int next_n = n, next_tile = tile;
+    for (; item < end; ++item, n = next_n, tile = next_tile) {
+        const int L = ahead.length, m = row_of(tile), m0 = (tile * NW + wave) * 32;
         Row row = make_row(A, ahead, m);
-        if (item + 1 < end) ahead = look_ahead(A, (item + 1) / A.tiles, (tile_of(item + 1) * NW + wave) * 32 + (lane & 31));
+        if (--next_tile < 0) {
+            next_tile = A.tiles - 1;
+            ++next_n;
+        }
+        if (item + 1 < end) ahead = look_ahead(A, next_n, row_of(next_tile));
         const BlockInfo blk = make_block(A, L, m0, row);
         row.pos = min(max(row.pos, blk.pos_lo), blk.pos_hi);  // also where there is no row
         if (lane == 0) {
@@ -126,7 +131,6 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
 
         float16_t dq[DP / 32];
         clear(dq);
-        bool careful = false;
         if (lo < hi) {
             ks.store(tiles, lo, hi, tid);
             vs.store(tiles + KT * DP, lo, hi, tid);
@@ -149,14 +153,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                     scale_scores(s, A.c, bias, A.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r] - top) * (dp[r] * inv - delta);
-                    if (key0 < blk.full_lo || key0 + 32 > blk.full_hi) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int key = key0 + mfma_row(r, half);
-                            s[r] = key >= row.lo && key < row.hi ? s[r] : 0.0f;
-                        }
-                        careful = careful || !finite_rows<T, DP>(kt, 32 * b, lane);
-                    }
+                    mask_keys(s, 0.0f, row, blk, key0, half);
                     if (bias) {
                         const int one = one_distance(key0, blk.pos_lo, blk.pos_hi, A.n_distances);
                         if (one >= 0) {
@@ -211,7 +208,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
             }
         }
         if (row.valid) store_row<T, DP>(A.dq.at<T>(n, row.i, head), dq, A.scale, A.dim, half);
-        if (careful) careful_dq<T>(A, n, g, L, m0, table, row, top, inv, delta, lane);
+        if (!all_finite(dq)) careful_dq<T>(A, n, g, L, m0, table, row, top, inv, delta, lane);
         __syncthreads();  // the next item overwrites what this one read
     }
     if (A.bias) {

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(64 * (TPR_WAVES > 1 ? TPR_WAVES : 4)) k_rms_no
     for (int x = threadIdx.x; x < a.width; x += blockDim.x) part[x] = columns[x];
 }
 
-// dweight from the blocks' parts: a block takes 4 columns, its threads 256 rows of parts at a time
+// The columns of blocks' parts [count][width] added up: a block takes 4 columns, its threads 256 parts at a time
 __global__ void __launch_bounds__(1024) k_column_sum(const float* parts, int count, int width, void* out, int type) {
     __shared__ float part[16][4];
     const int sub = threadIdx.x >> 2, col = blockIdx.x * 4 + (threadIdx.x & 3);
@@ -369,6 +369,11 @@ int widest(int width, int type) {
 }
 
 }  // namespace
+
+void column_sum(const float* parts, int count, int width, void* out, int type, hipStream_t st) {
+    hipLaunchKernelGGL(k_column_sum, dim3((width + 3) / 4), dim3(1024), 0, st, parts, count, width, out, type);
+}
+
 }  // namespace goi
 
 using namespace goi;
@@ -436,8 +441,7 @@ int32_t goi_rms_norm_backward(const GoiNormBackward* a, void* workspace, uint64_
         else if (a->type == GOI_F16) launch_backward<f16>(*a, vec, tpr, blocks, parts, st);
         else launch_backward<bf16>(*a, vec, tpr, blocks, parts, st);
     }
-    hipLaunchKernelGGL(k_column_sum, dim3((a->width + 3) / 4), dim3(1024), 0, st, parts, blocks, a->width, a->dweight,
-                       a->weight_type);
+    column_sum(parts, blocks, a->width, a->dweight, a->weight_type, st);
     return launch_error(who);
 }
 
