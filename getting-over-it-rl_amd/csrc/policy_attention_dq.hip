@@ -15,6 +15,37 @@ __device__ __forceinline__ void in_step() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// Adds up the columns of the skewed block's rows, a head's at a time, to the lane's distance of each head: all of the block's
+// reads are on their way at once
+template <int G>
+__device__ __forceinline__ void add_columns(const float* skew, float* sum, int table, int lane) {
+    float v[kSkewRows], t[G];
+#pragma unroll
+    for (int r = 0; r < kSkewRows; ++r) v[r] = skew[r * kSkew + lane];
+#pragma unroll
+    for (int hl = 0; hl < G; ++hl) t[hl] = sum[hl * table];
+#pragma unroll
+    for (int r = 0; r < kSkewRows; ++r) t[r % G] += v[r];
+#pragma unroll
+    for (int hl = 0; hl < G; ++hl) sum[hl * table] = t[hl];
+}
+// The same for any group; turn: the first row's head
+__device__ __forceinline__ void add_columns(const float* skew, float* sum, int table, int group, int turn, int lane) {
+    for (int hl = 0; hl < group; ++hl) {
+        int r = hl - turn;
+        r += r < 0 ? group : 0;
+        float t = 0.0f;
+#pragma unroll 4
+        for (; r < kSkewRows; r += group) t += skew[r * kSkew + lane];
+        sum[hl * table] += t;
+    }
+}
+__device__ __forceinline__ void clear_skew(float* skew, int lane) {
+#pragma unroll
+    for (int x = 0; x < kSkewRows * kSkew / 256; ++x)
+        reinterpret_cast<float4_t*>(skew)[x * 64 + lane] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
 // dq of a wave's 32 rows pair by pair
 template <typename T>
 __device__ void careful_dq(const AttnRun& A, int n, int g, int L, int m0, const float* table, const Row& mine, float my_top,
@@ -68,6 +99,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     Ahead ahead = look_ahead(A, n, row_of(tile));
     if (A.bias) {
         for (int x = lane; x < A.group * A.table; x += 64) sums[x] = 0.0f;
+        clear_skew(skew, lane);
         bl.stage(A, g, tid, NT);
     }
     int next_n = n, next_tile = tile;
@@ -168,24 +200,18 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                             float* const to = skew + (lane & 15) * kSkew + 31 - shift + 4 * half;
 #pragma unroll
                             for (int rows = 0; rows < 32; rows += kSkewRows) {
-#pragma unroll
-                                for (int x = 0; x < kSkewRows * kSkew / 256; ++x)
-                                    reinterpret_cast<float4_t*>(skew)[x * 64 + lane] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                                in_step();
                                 if ((lane & 16) == rows) {
 #pragma unroll
                                     for (int r = 0; r < 16; ++r) to[mfma_row(r, 0)] = s[r];
                                 }
                                 in_step();
-                                const int turn = (m0 + rows) % A.group;
-                                for (int hl = 0; hl < A.group; ++hl) {
-                                    int r = hl - turn;
-                                    r += r < 0 ? A.group : 0;
-                                    float t = 0.0f;
-#pragma unroll 4
-                                    for (; r < kSkewRows; r += A.group) t += skew[r * kSkew + lane];
-                                    sum[hl * A.table] += t;
-                                }
+                                if (A.group == 1) add_columns<1>(skew, sum, A.table, lane);
+                                else if (A.group == 2) add_columns<2>(skew, sum, A.table, lane);
+                                else if (A.group == 4) add_columns<4>(skew, sum, A.table, lane);
+                                else if (A.group == 8) add_columns<8>(skew, sum, A.table, lane);
+                                else add_columns(skew, sum, A.table, A.group, (m0 + rows) % A.group, lane);
+                                in_step();
+                                clear_skew(skew, lane);  // for the next rows
                                 in_step();
                             }
                         }
