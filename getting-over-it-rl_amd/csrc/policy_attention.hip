@@ -317,9 +317,9 @@ int check_sizes(const GoiAttention* a, AttnRun* A, const char* who) {
 // The items of a key head and the blocks that share them. Short windows: a block stages the bias once for many items, so the
 // blocks are those that the chip holds a few times over; long ones, whose items differ in size, go to blocks of their own.
 constexpr int kCus = 256, kCuLds = 160 * 1024;  // MI355X
-int share_items(AttnRun* A, int64_t items, int waves, size_t lds, const char* who, bool apart = false) {
+int share_items(AttnRun* A, int64_t items, int waves, size_t lds, const char* who, bool sums = false, bool apart = false) {
     const int64_t resident = kCus * std::max<int64_t>(1, std::min<int64_t>(8 / waves, kCuLds / (int64_t)(lds + 512)));
-    const int64_t want = A->k_steps >= 1024 || apart ? items : std::max<int64_t>(1, 3 * resident / A->kv_heads);
+    const int64_t want = (A->k_steps >= 1024 && !sums) || apart ? items : std::max<int64_t>(1, 3 * resident / A->kv_heads);
     const int64_t blocks = std::min(items, want);
     if (items > INT_MAX || blocks * A->kv_heads > INT_MAX) return policy_error(GOI_E_UNSUPPORTED, "%s: more than 2^31 tiles", who);
     A->items = (int)items;
@@ -365,7 +365,7 @@ int plan_backward(AttnRun* run, BackwardPlan* plan, const char* who) {
     A.tiles = (A.rows + 32 * p.waves - 1) / (32 * p.waves);
     // the bias' sums of a lane are of one head: items whose rows start at other heads are kept apart
     const int rc = share_items(run, (int64_t)a.n_worlds * A.tiles, p.waves, attention_dq_lds(A, p.waves), who,
-                               a.bias && 32 % A.group != 0);
+                               a.bias != nullptr, a.bias && 32 % A.group != 0);
     if (rc != GOI_OK) return rc;
     const uint64_t pairs = (uint64_t)a.n_worlds * a.kv_heads;
     p.blocks_at = round16(pairs * A.rows * sizeof(RowInfo));
