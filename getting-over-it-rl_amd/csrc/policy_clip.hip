@@ -10,7 +10,7 @@ namespace goi {
 namespace {
 
 constexpr int kTensors = 112;      // tables of 32 bytes a tensor within the 4 KB of kernel arguments
-constexpr int kSegment = 4096;     // elements of a tensor that a block takes at a time
+constexpr int kSegment = 8192;     // elements of a tensor that a block takes at a time
 constexpr int kBlocks = 2048;      // blocks of a launch, and partial sums it leaves: 8 a CU
 
 struct Tensors {
@@ -68,9 +68,7 @@ __device__ __forceinline__ double block_sum(double x, double* shared) {
 __global__ void __launch_bounds__(256) k_square_sums(const Tensors t, double* parts) {
     __shared__ double shared[4];
     double s = 0.0;
-    const int end = (int)((int64_t)(blockIdx.x + 1) * t.segments / gridDim.x);
-    int seg = (int)((int64_t)blockIdx.x * t.segments / gridDim.x);
-    for (int i = tensor_of(t, seg); seg < end; ++seg) {
+    for (int seg = blockIdx.x, i = tensor_of(t, seg); seg < t.segments; seg += gridDim.x) {
         while (i + 1 < t.count && t.first[i + 1] <= seg) ++i;
         const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
         const int n = (int)min((int64_t)kSegment, t.size[i] - at);
@@ -116,8 +114,8 @@ __device__ __forceinline__ void scale_to(const T* x, void* out, int type, int64_
     else scale(x, static_cast<bf16*>(out) + at, n, f);
 }
 
-// Each block sums the partial sums itself (a few KB from L2) in the same order. A block's segments run backwards, from those
-// that the pass before read last.
+// Each block sums the partial sums itself (a few KB from L2) in the same order. The segments run backwards, from those that
+// the pass before read last and the last-level cache may still hold.
 __global__ void __launch_bounds__(256) k_clip(const Tensors t, const double* parts, int count, float max_norm, float* norm) {
     __shared__ double shared[4];
     double s = 0.0;
@@ -126,9 +124,7 @@ __global__ void __launch_bounds__(256) k_clip(const Tensors t, const double* par
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = total;
     float f = max_norm / (total + 1e-6f);
     f = f > 1.0f ? 1.0f : f;
-    const int block = gridDim.x - 1 - blockIdx.x, begin = (int)((int64_t)block * t.segments / gridDim.x);
-    int seg = (int)((int64_t)(block + 1) * t.segments / gridDim.x) - 1;
-    for (int i = tensor_of(t, max(seg, 0)); seg >= begin; --seg) {
+    for (int seg = t.segments - 1 - (int)blockIdx.x, i = tensor_of(t, max(seg, 0)); seg >= 0; seg -= gridDim.x) {
         while (i > 0 && t.first[i] > seg) --i;
         if (t.out[i] == t.grad[i] && f == 1.0f) continue;
         const int64_t at = (int64_t)(seg - t.first[i]) * kSegment;
