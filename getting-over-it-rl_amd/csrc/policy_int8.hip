@@ -84,31 +84,39 @@ __global__ void __launch_bounds__(256) k_int8_few(const GoiInt8 a) {
     }
 }
 
-constexpr int kStep = 64;  // bytes of k a step
+constexpr int kStep = 64;    // bytes of k a step: two products' width
+constexpr int kBuffers = 3;  // steps in LDS
 
-// LDS of two tiles, or of the four waves' parts of the finished one
+// Waits until at most N of the wave's loads are on their way (some: they were issued), or none, and for the block
+template <int N>
+__device__ __forceinline__ void loads_left(bool some) {
+    if (some) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// LDS of the steps' tiles, or of the four waves' parts of the finished one
 template <typename T, int MB, int NB>
 constexpr int lds_tile() {
-    constexpr int a = 2 * 64 * (MB + NB) * kStep, b = (int)(4 * 32 * (32 * NB + 8) * sizeof(T));
+    constexpr int a = kBuffers * 64 * (MB + NB) * kStep, b = (int)(4 * 32 * (32 * NB + 8) * sizeof(T));
     return a > b ? a : b;
 }
 
 // Many rows: a block takes BM rows and BN channels, each of its four waves 32 MB rows x 32 NB channels of them, kStep bytes of k
-// a step through two LDS tiles. Memory goes straight to LDS, a wave's 1 KB at a time (16 rows): the next step's loads are in
-// flight while this one is multiplied, in no registers. The channels are the first operand, so that a lane's sums are of one row and
+// a step through three LDS tiles. Memory goes straight to LDS, a wave's 1 KB at a time (16 rows): the next two steps' loads are
+// in flight while one is multiplied, in no registers. The channels are the first operand, so that a lane's sums are of one row and
 // groups of four channels; the finished tile leaves through LDS in whole 16-byte pieces of rows.
 template <typename T, int MB, int NB>
 __global__ void __launch_bounds__(256, 2) k_int8(const GoiInt8 a, int tiles_n) {
-    constexpr int BM = 64 * MB, BN = 64 * NB, ROWS = BM + BN, PER = ROWS / 64;  // PER: loads of 16 rows a wave and step
-    extern __shared__ __attribute__((aligned(16))) char lds[];  // [2][BM rows of x, BN of w][kStep]
+    constexpr int BM = 64 * MB, BN = 64 * NB, ROWS = BM + BN, LPR = kStep / 16, RPL = 64 / LPR, PER = ROWS / (4 * RPL);
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // [kBuffers][BM rows of x, BN of w][kStep]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int place = xcd_place(blockIdx.x, gridDim.x);
     const int m0 = place / tiles_n * BM, n0 = place % tiles_n * BN;
-    // row r of the tile, chunk c of 16 bytes, lies at chunk_at<32>(r, c); a load's lane is a place, so it fetches the place's chunk
+    // row r of the tile, chunk c of 16 bytes, lies at chunk_at<kStep / 2>(r, c); a load's lane is a place, so it fetches the place's chunk
     const int8_t* from[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int r = (wave * PER + j) * 16 + (lane >> 2), ch = (lane & 3) ^ (chunk_at<32>(r, 0) & 3);
+        const int r = (wave * PER + j) * RPL + lane / LPR, ch = (lane % LPR) ^ (chunk_at<kStep / 2>(r, 0) % LPR);
         from[j] = (r < BM ? a.x + (int64_t)min(m0 + r, a.rows - 1) * a.x_stride
                           : a.w + (int64_t)min(n0 + r - BM, a.channels - 1) * a.w_stride) + 16 * ch;
     }
@@ -116,7 +124,7 @@ __global__ void __launch_bounds__(256, 2) k_int8(const GoiInt8 a, int tiles_n) {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from[j] + k0),
-                                             (__attribute__((address_space(3))) void*)(lds + (buf * ROWS + (wave * PER + j) * 16) * kStep),
+                                             (__attribute__((address_space(3))) void*)(lds + (buf * ROWS + (wave * PER + j) * RPL) * kStep),
                                              16, 0, 0);
     };
     int16v c[MB][NB];
@@ -127,44 +135,61 @@ __global__ void __launch_bounds__(256, 2) k_int8(const GoiInt8 a, int tiles_n) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) c[i][j][r] = 0;
     const int mw = (wave >> 1) * 32 * MB, nw = (wave & 1) * 32 * NB;  // the wave's part of the tile
-    const auto multiply = [&](int buf) {
-        const int4_t* const x = reinterpret_cast<const int4_t*>(lds + buf * ROWS * kStep);
-        const int4_t* const w = x + BM * (kStep / 16);
-#pragma unroll
-        for (int s = 0; s < kStep / 32; ++s) {
-            int4_t fx[MB], fw[NB];
-#pragma unroll
-            for (int i = 0; i < MB; ++i) fx[i] = x[chunk_at<32>(mw + 32 * i + (lane & 31), 2 * s + half)];
-#pragma unroll
-            for (int j = 0; j < NB; ++j) fw[j] = w[chunk_at<32>(nw + 32 * j + (lane & 31), 2 * s + half)];
-#pragma unroll
-            for (int i = 0; i < MB; ++i)
-#pragma unroll
-                for (int j = 0; j < NB; ++j) c[i][j] = mfma(fw[j], fx[i], c[i][j]);
-        }
+    struct Operands {
+        int4_t x[MB], w[NB];
     };
+    const auto read = [&](Operands& f, int buf, int s) {
+        const int4_t* const x = reinterpret_cast<const int4_t*>(lds + buf * ROWS * kStep);
+        const int4_t* const w = x + BM * LPR;
+#pragma unroll
+        for (int i = 0; i < MB; ++i) f.x[i] = x[chunk_at<kStep / 2>(mw + 32 * i + (lane & 31), 2 * s + half)];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) f.w[j] = w[chunk_at<kStep / 2>(nw + 32 * j + (lane & 31), 2 * s + half)];
+    };
+    const auto multiply = [&](const Operands& f) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) c[i][j] = mfma(f.w[j], f.x[i], c[i][j]);
+    };
+    Operands f0, f1;  // a step's two halves
     // what is left over of k first, byte by byte at the row's end, so that the steps that follow are whole
     const int rest = a.width % kStep;
     if (rest) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int r = (wave * PER + j) * 16 + (lane >> 2), ch = (lane & 3) ^ (chunk_at<32>(r, 0) & 3);
-            reinterpret_cast<int4_t*>(lds)[r * (kStep / 16) + (lane & 3)] =
+            const int r = (wave * PER + j) * RPL + lane / LPR, ch = (lane % LPR) ^ (chunk_at<kStep / 2>(r, 0) % LPR);
+            reinterpret_cast<int4_t*>(lds)[r * LPR + lane % LPR] =
                 row_bytes(from[j] - 16 * ch + a.width - rest, 16 * ch, rest);
         }
         __syncthreads();
-        multiply(0);
+        read(f0, 0, 0);
+        read(f1, 0, 1);
+        multiply(f0);
+        multiply(f1);
         __syncthreads();
     }
-    int buf = 0;
-    if (a.width >= kStep) load(0, 0);
+    // Step i is multiplied while the loads of i + 1 and i + 2 are on their way, and each half of a step while the next half's
+    // operands are read: a wave waits until the PER loads that it issued
+    // last are the only ones left, so its part of step i + 1 is in LDS, and after the barrier everybody's is; the buffer that i + 3
+    // then overwrites was read before that barrier.
+    const int steps = a.width / kStep;
+    if (steps > 0) load(0, 0);
+    if (steps > 1) load(kStep, 1);
+    loads_left<PER>(steps > 1);
+    if (steps > 0) read(f0, 0, 0);
+    for (int i = 0, buf = 0; i < steps; ++i) {
+        if (i + 2 < steps) load((i + 2) * kStep, buf == 0 ? 2 : buf - 1);
+        read(f1, buf, 1);
+        multiply(f0);
+        __builtin_amdgcn_sched_barrier(0);
+        loads_left<PER>(i + 2 < steps);
+        buf = buf == 2 ? 0 : buf + 1;
+        read(f0, buf, 0);  // past the last step: what an earlier one left there, not used
+        multiply(f1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
-    for (int k0 = kStep; k0 <= a.width - rest; k0 += kStep) {
-        if (k0 < a.width - rest) load(k0, buf ^ 1);
-        multiply(buf);
-        buf ^= 1;
-        __syncthreads();
-    }
     // the channels' scales and biases
     float* const scale = reinterpret_cast<float*>(lds + lds_tile<T, MB, NB>());
     float* const bias = scale + BN;
