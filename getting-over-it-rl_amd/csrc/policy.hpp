@@ -166,4 +166,13 @@ __device__ __forceinline__ half8<T> to_operand(const float16_t& c, int x) {
     return __builtin_convertvector(f, half8<T>);
 }
 
+// What to_operand's rounding left of those registers, rounded in its turn
+template <typename T>
+__device__ __forceinline__ half8<T> rest_operand(const float16_t& c, int x, half8<T> rounded) {
+    float8_t f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = c[8 * x + e] - (float)rounded[e];
+    return __builtin_convertvector(f, half8<T>);
+}
+
 }  // namespace goi

@@ -157,9 +157,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                 inv = 1.0f / st.y;
             }
             delta = inv != 0.0f ? delta * inv : 0.0f;
-            if (row.valid && half == 0)
-                A.row_info[(int64_t)(n * A.kv_heads + g) * A.rows + m] = RowInfo{top, inv, delta, row.lo, row.hi};
         }
+        float slip = 0.0f;  // sum of the row's dS
 
         float16_t dq[DP / 32];
         clear(dq);
@@ -186,6 +185,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r] - top) * (dp[r] * inv - delta);
                     mask_keys(s, 0.0f, row, blk, key0, half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) slip += s[r];
                     if (bias) {
                         const int one = one_distance(key0, blk.pos_lo, blk.pos_hi, A.n_distances);
                         if (one >= 0) {
@@ -218,10 +219,17 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
+                        // dS rounded once costs dq as much precision as its own rounding does: up to 64 elements, where the
+                        // second product costs 3%, what the first left follows (at 128 it would cost 29%, in spilled registers)
                         const half8<T> ds = to_operand<T>(s, x);
+                        half8<T> rest;
+                        if constexpr (DP < 128) rest = rest_operand<T>(s, x, ds);
 #pragma unroll
-                        for (int d = 0; d < DP / 32; ++d)
-                            dq[d] = mfma(column_fragment<T, DP>(kt, 32 * b + 16 * x, 32 * d, lane), ds, dq[d]);
+                        for (int d = 0; d < DP / 32; ++d) {
+                            const half8<T> f = column_fragment<T, DP>(kt, 32 * b + 16 * x, 32 * d, lane);
+                            dq[d] = mfma(f, ds, dq[d]);
+                            if constexpr (DP < 128) dq[d] = mfma(f, rest, dq[d]);
+                        }
                     }
                 }
                 if (NBUF == 1) __syncthreads();
@@ -233,6 +241,11 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                 __syncthreads();
             }
         }
+        // A row's dS add up to 0 but for the error of delta, which comes from an output whose sums and itself were rounded: the
+        // pass over keys gets the delta with which they do.
+        slip = half_sum(slip);
+        if (row.valid && half == 0)
+            A.row_info[(int64_t)(n * A.kv_heads + g) * A.rows + m] = RowInfo{top, inv, delta + slip * inv, row.lo, row.hi};
         if (row.valid) store_row<T, DP>(A.dq.at<T>(n, row.i, head), dq, A.scale, A.dim, half);
         if (!all_finite(dq)) careful_dq<T>(A, n, g, L, m0, table, row, top, inv, delta, lane);
         __syncthreads();  // the next item overwrites what this one read
