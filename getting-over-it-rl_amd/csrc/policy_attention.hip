@@ -38,8 +38,15 @@ __device__ void careful_rows(const AttnRun& A, int n, int g, int L, int split, i
     }
 }
 
+// out = sum_j 2^(s_j - M) v_j / sum_j 2^(s_j - M) in one pass over the keys, M and the sum running along in float32.
 // NW waves of 32 packed rows each share tiles of KT keys. Two tiles of LDS (one for a single wave, which needs no barrier):
-// the next tile's loads are in flight while this one is computed.
+// the next tile's loads are in flight while this one is computed. The keys are the first operand, so a lane's scores are
+// of ONE row: its maximum and sum need one exchange between the lane's halves, and P rounds into the second product's operand
+// where it stands. Few rows (acting) take one wave and, until the chip is full, splits of the key axis.
+// Bound by the vector unit where rows are many (the softmax and the bias' lookup, some 10 operations a pair), by memory where
+// they are few. Measured in bfloat16, with bias: 4,096 windows of 128 steps with episodes, 8 heads of 64 on 2, 503 us (1.37 GB);
+// 8 windows of 4,001 steps, 16 heads of 128 on 4, 426 us (279 GFLOP, 655 TFLOP/s); one step each over 16,384 caches of up to 128
+// steps, 8 heads of 64 on 2, 143 us (0.54 GB, 3,760 GB/s, where a copy reaches 5,160).
 template <typename T, int DP, int NW, bool kSplit>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 || NW < 4 ? 2 : 3) k_attention(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
@@ -203,7 +210,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 
 }
 
 // Joins the splits of each row: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, M the largest m_s. A block a row, its
-// waves a quarter of the splits each.
+// waves a quarter of the splits each. Bound by latency: 11 us for the 192 rows of 12 caches of up to 65,536 steps, whose splits
+// take 117 us (0.38 GB, 3,230 GB/s); 3 us for one world's 8 rows.
 template <typename T>
 __global__ void __launch_bounds__(256) k_attention_join(const AttnRun A) {
     __shared__ float4_t shared[4][64];

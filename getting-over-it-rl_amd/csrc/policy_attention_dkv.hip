@@ -108,6 +108,11 @@ __device__ void careful_keys(const AttnRun& A, int n, int g, int L, int key0, co
     }
 }
 
+// Four products a pair. A block's keys are 32 a wave, and each tile of rows that it loads serves them all; blocks of the later
+// keys of a causal window have fewer rows and go last. Bound by latency between the products and the vector unit: at dim 128 dk and
+// dv fill half the registers, one wave a SIMD runs, and nothing else fills its waits (a second buffer of rows hides memory's).
+// Measured in bfloat16, with bias: 4,096 windows of 128 steps, 8 heads of 64 on 2, 739 us (1.6 GB); 8 windows of 4,001 steps, 16
+// heads of 128 on 4, 1,418 us (558 GFLOP, 394 TFLOP/s).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(const AttnRun A) {
     constexpr int NT = 64 * NW, RT = tile_rows(DP, NW), RB = RT / 32, NBUF = tile_buffers(NW);

@@ -36,15 +36,16 @@ extern "C" {
  *       out = sum_j softmax(s)_j v_j,     stats = { M, sum_j 2^(s_j log2(e) - M) } with M = max_j s_j log2(e)
  *   (two numbers and not the logarithm of the sum, which would lose the sum where M is a mask's -3e38). A query that sees
  *   no key, or only scores of minus infinity, gives out = 0 and stats = { minus infinity, 0 }, and no gradient.
- *   Keys and values that no query sees may hold anything, NaN and infinities among them, and are not read past L.
+ *   Keys and values that no query sees may hold anything, NaN and infinities among them, and are not read past L. A value that is
+ *   not finite reaches the results of the queries that see it, and in the backward call of the keys these see, and no others.
  *
  * Products are of the 16-bit inputs with float32 sums; the maximum, the sum and the accumulators of the softmax are float32;
  * probabilities and their gradients are rounded to the inputs' type for the second products.
  *
  * Limits: type GOI_BF16 or GOI_F16; dim a multiple of 8, 8 .. 128; 16-byte aligned pointers and strides (elements) that are
- * multiples of 8 (steps and heads within 0 .. 2^24), the last axis contiguous; n_buckets <= 64; group * (n_distances + 128) <= 6144. A bucket outside 0 .. n_buckets - 1 is
- * taken as the nearest one. bias_type is type or GOI_F32. stats is [n_worlds, heads, q_steps, 2] contiguous and may be null in the
- * forward call. */
+ * multiples of 8 (steps and heads within 0 .. 2^24), the last axis contiguous; n_buckets <= 64; group * (n_distances + 128) <=
+ * 6144; q_steps * group^2 < 2^32. A bucket outside 0 .. n_buckets - 1 is taken as the nearest one. bias_type is type or GOI_F32.
+ * stats is [n_worlds, heads, q_steps, 2] contiguous and may be null in the forward call. */
 typedef struct GoiAttention {
     int32_t n_worlds, q_steps, k_steps, heads, kv_heads, dim;
     int32_t type;   /* GOI_BF16 or GOI_F16: q, k, v, out and their gradients */
