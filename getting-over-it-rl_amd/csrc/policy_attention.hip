@@ -57,31 +57,18 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 
     const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
-    const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
-    // the later row tiles of a causal window see the most keys: they go first
-    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    int item = (int)((int64_t)block * A.items / A.per_head);
-    int n = item / A.tiles, tile = A.tiles - 1 - (item - n * A.tiles), split = 0;
-    if (kSplit) {
-        const int x = n / A.splits;
-        split = n - x * A.splits;
-        n = x;
-    }
+    // the later row tiles of a causal window see the most keys
+    Items<true> items(A);
+    const int g = items.g;
     const auto row_of = [&](int tile) { return (tile * NW + wave) * 32 + (lane & 31); };
-    Ahead ahead = look_ahead(A, n, row_of(tile));
+    Ahead ahead = look_ahead(A, items.n, row_of(items.tile));
     if (A.bias) bl.stage(A, g, tid, NT);
-    int next_n = n, next_tile = tile, next_split = split;
-    for (; item < end; ++item, n = next_n, tile = next_tile, split = next_split) {
+    while (items.more()) {
+        const int n = items.n, tile = items.tile, split = kSplit ? items.split : 0;
         const int L = ahead.length, m = row_of(tile), m0 = (tile * NW + wave) * 32;
         Row row = make_row(A, ahead, m);
-        if (--next_tile < 0) {
-            next_tile = A.tiles - 1;
-            if (!kSplit || ++next_split == A.splits) {
-                next_split = 0;
-                ++next_n;
-            }
-        }
-        if (item + 1 < end) ahead = look_ahead(A, next_n, row_of(next_tile));
+        items.next(A);
+        if (items.more()) ahead = look_ahead(A, items.n, row_of(items.tile));
         if (kSplit) {
             row.lo = max(row.lo, split * A.span);
             row.hi = min(row.hi, (split + 1) * A.span);
@@ -323,12 +310,16 @@ int check_sizes(const GoiAttention* a, AttnRun* A, const char* who) {
 }
 
 // The items of a key head and the blocks that share them. Short windows: a block stages the bias once for many items, so the
-// blocks are those that the chip holds a few times over; long ones, whose items differ in size, go to blocks of their own.
+// blocks are those that the chip holds a few times over; long ones, whose items differ in size, go to blocks of their own,
+// or, with sums that a block ends with, to as many blocks as for short ones, largest first.
 constexpr int kCus = 256, kCuLds = 160 * 1024;  // MI355X
 int share_items(AttnRun* A, int64_t items, int waves, size_t lds, const char* who, bool sums = false, bool apart = false) {
     const int64_t resident = kCus * std::max<int64_t>(1, std::min<int64_t>(8 / waves, kCuLds / (int64_t)(lds + 512)));
     const int64_t want = (A->k_steps >= 1024 && !sums) || apart ? items : std::max<int64_t>(1, 3 * resident / A->kv_heads);
-    const int64_t blocks = std::min(items, want);
+    int64_t blocks = std::min(items, want);
+    A->spread = A->k_steps >= 1024;
+    // an odd number, so that a block's items are not all of one world where the worlds are a power of two
+    if (A->spread && blocks < items && blocks > 1) blocks -= 1 - blocks % 2;
     if (items > INT_MAX || blocks * A->kv_heads > INT_MAX) return policy_error(GOI_E_UNSUPPORTED, "%s: more than 2^31 tiles", who);
     A->items = (int)items;
     A->per_head = (int)blocks;

@@ -58,6 +58,7 @@ struct AttnRun {
     int tiles;            // row tiles (forward, dq) or key tiles (dkv) of a key head
     int items;            // tiles (and splits) of all the worlds' windows with one key head, shared out over `per_head` blocks
     int per_head;
+    int spread;  // 0: a block takes neighbouring items; 1: every per_head-th one (Items)
     int splits;  // forward: the key axis is cut into `splits` ranges of `span` keys, joined afterwards
     int span;
     int origin;  // index of distance 0 in buckets
@@ -90,6 +91,61 @@ __device__ __forceinline__ int step_of(const AttnRun& A, int m) {
 __device__ __forceinline__ int history(const AttnRun& A, int n) {
     return A.lengths ? min(max(A.lengths[n], 0), A.k_steps) : A.k_steps;
 }
+
+// The items of a block, an item being a tile of rows or keys of a world's window (and a split of the keys), and the one it is at.
+// Short windows: neighbours, so that the tiles of a window follow one another. Long ones differ in size, by their place in a causal
+// window and by the episodes and histories of their worlds: the largest tiles of all worlds go first, and the worlds take turns, so that
+// each block and each of the 8 XCDs, to which the blocks are dealt in turn, gets its share of every world.
+// kLast: a window's last tiles are its largest (rows), otherwise its first (keys).
+template <bool kLast>
+struct Items {
+    int g, block;
+    int n, tile, split;
+    int item, end;
+    __device__ __forceinline__ explicit Items(const AttnRun& A) {
+        if (A.spread) {
+            block = blockIdx.x / (uint32_t)A.kv_heads;
+            g = blockIdx.x - block * A.kv_heads;
+            item = block;
+            end = A.items;
+        } else {
+            const int place = xcd_place(blockIdx.x, gridDim.x);
+            g = place / A.per_head;
+            block = place - g * A.per_head;
+            item = (int)((int64_t)block * A.items / A.per_head);
+            end = (int)((int64_t)(block + 1) * A.items / A.per_head);
+            const int x = item / A.tiles;
+            tile = item - x * A.tiles;
+            n = x / A.splits;
+            split = x - n * A.splits;
+        }
+        if (A.spread) locate(A);
+        else if (kLast) tile = A.tiles - 1 - tile;
+    }
+    __device__ __forceinline__ void locate(const AttnRun& A) {
+        const uint32_t rank = (uint32_t)item / (uint32_t)A.n_worlds;
+        n = (uint32_t)((uint32_t)item - rank * A.n_worlds + rank) % (uint32_t)A.n_worlds;
+        split = rank / (uint32_t)A.tiles;
+        tile = rank - split * A.tiles;
+        if (kLast) tile = A.tiles - 1 - tile;
+    }
+    __device__ __forceinline__ bool more() const { return item < end; }
+    __device__ __forceinline__ void next(const AttnRun& A) {
+        if (A.spread) {
+            item = min((int64_t)item + A.per_head, (int64_t)INT_MAX);
+            if (item < end) locate(A);
+            return;
+        }
+        ++item;
+        if (kLast ? --tile < 0 : ++tile == A.tiles) {
+            tile = kLast ? A.tiles - 1 : 0;
+            if (++split == A.splits) {
+                split = 0;
+                ++n;
+            }
+        }
+    }
+};
 
 struct Row {
     bool valid;  // m < rows

@@ -123,12 +123,12 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
     const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
-    const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
+    Items<false> items(A);  // the first keys of a causal window are seen by the most rows
+    const int g = items.g;
     if (A.bias) bl.stage(A, g, tid, NT);
     RowStage<T, DP, RT, NT> stage(A, tid);
-    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    for (int item = (int)((int64_t)block * A.items / A.per_head); item < end; ++item) {
-        const int n = item / A.tiles, tile = item - n * A.tiles;  // the first keys are seen by the most rows: they go first
+    for (; items.more(); items.next(A)) {
+        const int n = items.n, tile = items.tile;
         const int L = history(A, n);
         const int block0 = tile * 32 * NW, block1 = min(block0 + 32 * NW, L);  // the block's keys
         const int key0 = block0 + wave * 32, key = key0 + (lane & 31);

@@ -86,7 +86,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     const float* const table = bl.table;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
 
-    const int place = xcd_place(blockIdx.x, gridDim.x), g = place / A.per_head, block = place - g * A.per_head;
+    Items<true> items(A);
+    const int g = items.g, first_tile = items.tile;
     // The bias' gradient: each wave adds up its pairs by head and distance, sums [group][A.table], like the table. A near block
     // goes through `skew`, 16 rows at a time, each row shifted by its position, so that a column holds one distance: a lane adds up
     // the columns of one distance, a head's rows at a time. (Adding each pair to its sum by LDS atomics took six times as long.)
@@ -97,25 +98,19 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     float far[2] = {0.0f, 0.0f};
     // a lane's rows are of the same head, and shifted alike, in all of a block's items (the host gives a block one item where
     // they are not)
-    const int end = (int)((int64_t)(block + 1) * A.items / A.per_head);
-    int item = (int)((int64_t)block * A.items / A.per_head);
-    int n = item / A.tiles, tile = A.tiles - 1 - (item - n * A.tiles);
     const auto row_of = [&](int tile) { return (tile * NW + wave) * 32 + (lane & 31); };
-    Ahead ahead = look_ahead(A, n, row_of(tile));
+    Ahead ahead = look_ahead(A, items.n, row_of(items.tile));
     if (A.bias) {
         for (int x = lane; x < A.group * A.table; x += 64) sums[x] = 0.0f;
         clear_skew(skew, lane);
         bl.stage(A, g, tid, NT);
     }
-    int next_n = n, next_tile = tile;
-    for (; item < end; ++item, n = next_n, tile = next_tile) {
+    while (items.more()) {
+        const int n = items.n, tile = items.tile;
         const int L = ahead.length, m = row_of(tile), m0 = (tile * NW + wave) * 32;
         Row row = make_row(A, ahead, m);
-        if (--next_tile < 0) {
-            next_tile = A.tiles - 1;
-            ++next_n;
-        }
-        if (item + 1 < end) ahead = look_ahead(A, next_n, row_of(next_tile));
+        items.next(A);
+        if (items.more()) ahead = look_ahead(A, items.n, row_of(items.tile));
         const BlockInfo blk = make_block(A, L, m0, row);
         row.pos = min(max(row.pos, blk.pos_lo), blk.pos_hi);  // also where there is no row
         if (lane == 0) {
@@ -257,7 +252,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
     }
     if (A.bias) {
         // the rows' far sums to the ends of their heads (an end's entries in the padding are the end's too)
-        const int m0 = (A.tiles - 1 - (int)((int64_t)block * A.items / A.per_head) % A.tiles) * NW * 32 + wave * 32;
+        const int m0 = (first_tile * NW + wave) * 32;
         skew[lane] = half_sum(far[0]);
         skew[64 + lane] = half_sum(far[1]);
         in_step();
@@ -282,7 +277,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
         }
         __syncthreads();
         // each sum by several threads, a range of distances each, where there are threads to spare
-        float* const part = A.part_bias + (int64_t)block * A.heads * A.n_buckets + g * A.group * A.n_buckets;
+        float* const part = A.part_bias + (int64_t)items.block * A.heads * A.n_buckets + g * A.group * A.n_buckets;
         const int outs = A.group * A.n_buckets, parts = max(1, NT / outs);
         const int ends = A.causal ? min(A.table, kPad + A.k_steps) : A.table;  // no causal pair is further apart
         for (int x = tid; x < outs * parts; x += NT) {
