@@ -44,8 +44,8 @@ __device__ void careful_rows(const AttnRun& A, int n, int g, int L, int split, i
 // of ONE row: its maximum and sum need one exchange between the lane's halves, and P rounds into the second product's operand
 // where it stands. Few rows (acting) take one wave and, until the chip is full, splits of the key axis.
 // Bound by the vector unit where rows are many (the softmax and the bias' lookup, some 10 operations a pair), by memory where
-// they are few. Measured in bfloat16, with bias: 4,096 windows of 128 steps with episodes, 8 heads of 64 on 2, 503 us (1.37 GB);
-// 8 windows of 4,001 steps, 16 heads of 128 on 4, 426 us (279 GFLOP, 655 TFLOP/s); one step each over 16,384 caches of up to 128
+// they are few. Measured in bfloat16, with bias: 4,096 windows of 128 steps with episodes, 8 heads of 64 on 2, 485 us (1.37 GB);
+// 8 windows of 4,001 steps, 16 heads of 128 on 4, 405 us (279 GFLOP, 690 TFLOP/s); one step each over 16,384 caches of up to 128
 // steps, 8 heads of 64 on 2, 143 us (0.54 GB, 3,760 GB/s, where a copy reaches 5,160).
 template <typename T, int DP, int NW, bool kSplit>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 || NW < 4 ? 2 : 3) k_attention(const AttnRun A) {
@@ -492,7 +492,7 @@ int32_t goi_attention_backward(const GoiAttention* a, void* workspace, uint64_t 
         int waves = std::max(least, waves_for(a->k_steps));
         while (waves > least && pairs * ((a->k_steps + 32 * waves - 1) / (32 * waves)) < 512) waves /= 2;
         A.tiles = (a->k_steps + 32 * waves - 1) / (32 * waves);
-        rc = share_items(&A, (int64_t)a->n_worlds * A.tiles, waves, attention_lds(A, waves), who);
+        rc = share_items(&A, (int64_t)a->n_worlds * A.tiles, waves, attention_dkv_lds(A, waves), who);
         if (rc != GOI_OK) return rc;
         e = launch_attention_dkv(A, waves, st);
         if (e != hipSuccess) return policy_error(GOI_E_HIP, "%s: %s", who, hipGetErrorString(e));

@@ -77,6 +77,8 @@ inline int attention_dim_tile(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 
 // thread holds few chunks of the next tile. Two tiles of LDS for blocks of several waves; a single wave needs no barrier and
 // overwrites its own.
 constexpr int tile_rows(int dp, int waves) { return dp == 128 || waves == 1 ? 32 : 64; }
+// The pass over keys takes 64 rows of 128 elements too where four waves share them: one block of them fills a CU's registers
+constexpr int key_pass_rows(int dp, int waves) { return waves == 4 ? 64 : tile_rows(dp, waves); }
 constexpr int tile_buffers(int waves) { return waves == 1 ? 1 : 2; }
 hipError_t launch_attention_dq(const AttnRun& A, int waves, hipStream_t st);
 hipError_t launch_attention_dkv(const AttnRun& A, int waves, hipStream_t st);
@@ -304,6 +306,10 @@ __host__ __device__ inline size_t bias_lds(const AttnRun& A) {
 inline size_t attention_lds(const AttnRun& A, int waves) {
     const int dp = attention_dim_tile(A.dim);
     return (size_t)tile_buffers(waves) * 2 * tile_rows(dp, waves) * dp * 2 + bias_lds(A);
+}
+inline size_t attention_dkv_lds(const AttnRun& A, int waves) {
+    const int dp = attention_dim_tile(A.dim);
+    return (size_t)tile_buffers(waves) * 2 * key_pass_rows(dp, waves) * dp * 2 + bias_lds(A);
 }
 // and of the pass over rows: each wave's skewed block and sums by distance (policy_attention_dq.hip)
 constexpr int kSkew = 64, kSkewRows = 16;  // words of a row of the skewed block; it is taken in halves

@@ -74,8 +74,8 @@ __device__ void careful_dq(const AttnRun& A, int n, int g, int L, int m0, const 
 // The forward kernel's split and layouts (lane = row), with dq as its sum and no running maximum. Three products a pair; dS goes
 // into the third in two parts, rounded and rest, where dim leaves room (DP < 128), so that dq keeps its own rounding's precision.
 // Bound by the vector unit: about 9 operations a pair for P and dS, 4 more and an LDS round trip for the bias' gradient near the
-// diagonal. Measured in bfloat16, with the bias' gradient: 4,096 windows of 128 steps, 8 heads of 64 on 2, 906 us (2.4 GB); 8
-// windows of 4,001 steps, 16 heads of 128 on 4, 812 us (419 GFLOP, 515 TFLOP/s).
+// diagonal. Measured in bfloat16, with the bias' gradient: 4,096 windows of 128 steps, 8 heads of 64 on 2, 880 us (2.4 GB); 8
+// windows of 4,001 steps, 16 heads of 128 on 4, 800 us (419 GFLOP, 524 TFLOP/s).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_attention_dq(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
