@@ -72,10 +72,10 @@ __device__ void careful_dq(const AttnRun& A, int n, int g, int L, int m0, const 
 }
 
 // The forward kernel's split and layouts (lane = row), with dq as its sum and no running maximum. Three products a pair; dS goes
-// into the third in two parts, rounded and rest, where dim leaves room (DP < 128), so that dq keeps its own rounding's precision.
+// into the third in two parts, rounded and rest, so that dq keeps its own rounding's precision.
 // Bound by the vector unit: about 9 operations a pair for P and dS, 4 more and an LDS round trip for the bias' gradient near the
 // diagonal. Measured in bfloat16, with the bias' gradient: 4,096 windows of 128 steps, 8 heads of 64 on 2, 880 us (2.4 GB); 8
-// windows of 4,001 steps, 16 heads of 128 on 4, 800 us (419 GFLOP, 524 TFLOP/s).
+// windows of 4,001 steps, 16 heads of 128 on 4, 950 us (419 GFLOP and the rest's 140; 800 us without it).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_attention_dq(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
@@ -219,16 +219,14 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        // dS rounded once costs dq as much precision as its own rounding does: up to 64 elements, where the
-                        // second product costs 3%, what the first left follows (at 128 it would cost 29%, in spilled registers)
-                        const half8<T> ds = to_operand<T>(s, x);
-                        half8<T> rest;
-                        if constexpr (DP < 128) rest = rest_operand<T>(s, x, ds);
+                        // dS rounded once costs dq as much precision as its own rounding does, so what the first product left
+                        // follows in a second
+                        const half8<T> ds = to_operand<T>(s, x), rest = rest_operand<T>(s, x, ds);
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) {
                             const half8<T> f = column_fragment<T, DP>(kt, 32 * b + 16 * x, 32 * d, lane);
                             dq[d] = mfma(f, ds, dq[d]);
-                            if constexpr (DP < 128) dq[d] = mfma(f, rest, dq[d]);
+                            dq[d] = mfma(f, rest, dq[d]);
                         }
                     }
                 }
