@@ -74,8 +74,8 @@ __device__ void careful_dq(const AttnRun& A, int n, int g, int L, int m0, const 
 // The forward kernel's split and layouts (lane = row), with dq as its sum and no running maximum. Three products a pair; dS goes
 // into the third in two parts, rounded and rest, so that dq keeps its own rounding's precision.
 // Bound by the vector unit: about 9 operations a pair for P and dS, 4 more and an LDS round trip for the bias' gradient near the
-// diagonal. Measured in bfloat16, with the bias' gradient: 4,096 windows of 128 steps, 8 heads of 64 on 2, 880 us (2.4 GB); 8
-// windows of 4,001 steps, 16 heads of 128 on 4, 950 us (419 GFLOP and the rest's 140; 800 us without it).
+// diagonal. Measured in bfloat16, with the bias' gradient: 4,096 windows of 128 steps, 8 heads of 64 on 2, 895 us (2.4 GB); 8
+// windows of 4,001 steps, 16 heads of 128 on 4, 807 us (419 GFLOP, 520 TFLOP/s, and the rest's 140).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_attention_dq(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
@@ -180,7 +180,9 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                     const int key0 = k0 + 32 * b;
                     if (key0 >= blk.hi || key0 + 32 <= blk.lo) continue;
                     float16_t s = raw_scores<T, DP>(kt, 32 * b, q, lane);
+                    if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);  // one product's operands at a time: registers
                     const float16_t dp = raw_scores<T, DP>(vt, 32 * b, go, lane);
+                    if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);
                     scale_scores(s, A.c, bias, A.n_distances, key0, row.pos, blk.pos_lo, blk.pos_hi, half);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r] - top) * (dp[r] * inv - delta);
@@ -222,12 +224,15 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : 2) k_atten
                         // dS rounded once costs dq as much precision as its own rounding does, so what the first product left
                         // follows in a second
                         const half8<T> ds = to_operand<T>(s, x), rest = rest_operand<T>(s, x, ds);
+                        // first all of the one, then all of the other: a product waits for the sums that it adds to (923 us
+                        // where each rest's follows at once and this takes 807)
+                        half8<T> f[DP / 32];
 #pragma unroll
-                        for (int d = 0; d < DP / 32; ++d) {
-                            const half8<T> f = column_fragment<T, DP>(kt, 32 * b + 16 * x, 32 * d, lane);
-                            dq[d] = mfma(f, ds, dq[d]);
-                            dq[d] = mfma(f, rest, dq[d]);
-                        }
+                        for (int d = 0; d < DP / 32; ++d) f[d] = column_fragment<T, DP>(kt, 32 * b + 16 * x, 32 * d, lane);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) dq[d] = mfma(f[d], ds, dq[d]);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) dq[d] = mfma(f[d], rest, dq[d]);
                     }
                 }
                 if (NBUF == 1) __syncthreads();
