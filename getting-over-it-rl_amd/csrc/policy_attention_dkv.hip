@@ -110,13 +110,14 @@ __device__ void careful_keys(const AttnRun& A, int n, int g, int L, int key0, co
 
 // Four products a pair. A block's keys are 32 a wave, and each tile of rows that it loads serves them all. Bound by latency between
 // the products and the vector unit: at dim 128 dk and dv fill a third of the registers, one wave a SIMD runs, and nothing else fills
-// its waits. Hence the operands read early (1,047 us where without 1,149 at dim 128; 678 and 719 at 64) and tiles of 64 rows.
-// Measured in bfloat16, with bias: 4,096 windows of 128 steps, 8 heads of 64 on 2, 690 us (1.6 GB); 8 windows of 4,001 steps, 16
-// heads of 128 on 4, 1,030 us (558 GFLOP, 540 TFLOP/s).
+// its waits. Hence the operands read early (at dim 128 975 us with half of them, 935 with all; 1,149 without where half took 1,047;
+// at 64 719 without and 678 with one of four) and tiles of 64 rows. Measured in bfloat16, with bias: 4,096 windows of 128 steps, 8
+// heads of 64 on 2, 704 us (1.6 GB); 8 windows of 4,001 steps, 16 heads of 128 on 4, 935 us (558 GFLOP, 597 TFLOP/s).
 template <typename T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(const AttnRun A) {
     constexpr int NT = 64 * NW, RT = key_pass_rows(DP, NW), RB = RT / 32, NBUF = tile_buffers(NW);
-    constexpr bool kEarly = DP != 64 || NW == 4;  // where registers are left for it
+    // of the second products' two halves, those whose operands are read early (at 64 both of dv's or one of dk's spill)
+    constexpr int kEarlyV = DP == 128 ? 2 : DP != 64 || NW == 4 ? 1 : 0, kEarlyK = DP == 128 ? 2 : 0;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ __attribute__((aligned(16))) RowValues<RT> values[NBUF];
     T* const tiles = reinterpret_cast<T*>(lds);  // [NBUF][q, dout][RT][DP]
@@ -228,13 +229,14 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                 if (m0 / 32 + b >= A.blocks || blk[b].lo >= key0 + 32 || blk[b].hi <= key0) continue;
                 float16_t p = raw_scores<T, DP>(qt, 32 * b, k, lane);
                 float16_t ds = raw_scores<T, DP>(gt, 32 * b, v, lane);
-                // the first of the next products' operands, on their way while P and dS are computed
-                half8<T> early_v[DP / 32], early_k[DP / 32];
-                if constexpr (kEarly)
+                // the next products' operands, as many as registers are left for, on their way while P and dS are computed
+                half8<T> early_v[2][DP / 32], early_k[2][DP / 32];
+#pragma unroll
+                for (int x2 = 0; x2 < 2; ++x2)
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        early_v[d] = column_fragment<T, DP>(gt, 32 * b, 32 * d, lane);
-                        if constexpr (DP == 128) early_k[d] = column_fragment<T, DP>(qt, 32 * b, 32 * d, lane);
+                        if (x2 < kEarlyV) early_v[x2][d] = column_fragment<T, DP>(gt, 32 * b + 16 * x2, 32 * d, lane);
+                        if (x2 < kEarlyK) early_k[x2][d] = column_fragment<T, DP>(qt, 32 * b + 16 * x2, 32 * d, lane);
                     }
                 const int r0 = 32 * b + 4 * half;  // the lane's rows: r0 + 8 x + 0 .. 3
                 const int a0 = min(max(blk[b].pos_lo - (key0 + 31), 0), A.n_distances - 1);
@@ -294,9 +296,8 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? 1 : 2) k_attention_dkv(co
                     const half8<T> pf = to_operand<T>(p, x2), sf = to_operand<T>(ds, x2);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        const bool ev = kEarly && x2 == 0, ek = ev && DP == 128;
-                        dv[d] = mfma(ev ? early_v[d] : column_fragment<T, DP>(gt, 32 * b + 16 * x2, 32 * d, lane), pf, dv[d]);
-                        dk[d] = mfma(ek ? early_k[d] : column_fragment<T, DP>(qt, 32 * b + 16 * x2, 32 * d, lane), sf, dk[d]);
+                        dv[d] = mfma(x2 < kEarlyV ? early_v[x2][d] : column_fragment<T, DP>(gt, 32 * b + 16 * x2, 32 * d, lane), pf, dv[d]);
+                        dk[d] = mfma(x2 < kEarlyK ? early_k[x2][d] : column_fragment<T, DP>(qt, 32 * b + 16 * x2, 32 * d, lane), sf, dk[d]);
                     }
                 }
             }
