@@ -44,9 +44,9 @@ __device__ void careful_rows(const AttnRun& A, int n, int g, int L, int split, i
 // of ONE row: its maximum and sum need one exchange between the lane's halves, and P rounds into the second product's operand
 // where it stands. Few rows (acting) take one wave and, until the chip is full, splits of the key axis.
 // Bound by the vector unit where rows are many (the softmax and the bias' lookup, some 10 operations a pair), by memory where
-// they are few. Measured in bfloat16, with bias: 4,096 windows of 128 steps with episodes, 8 heads of 64 on 2, 485 us (1.37 GB);
-// 8 windows of 4,001 steps, 16 heads of 128 on 4, 405 us (279 GFLOP, 690 TFLOP/s); one step each over 16,384 caches of up to 128
-// steps, 8 heads of 64 on 2, 143 us (0.54 GB, 3,760 GB/s, where a copy reaches 5,160).
+// they are few. Measured in bfloat16, with bias: 4,096 windows of 128 steps with episodes, 8 heads of 64 on 2, 515 us (1.37 GB);
+// 8 windows of 4,001 steps, 16 heads of 128 on 4, 458 us (279 GFLOP, 610 TFLOP/s, and the rest's 140; 400 us without it); one step
+// each over 16,384 caches of up to 128 steps, 8 heads of 64 on 2, 141 us (0.54 GB, 3,810 GB/s, where a copy reaches 5,020).
 template <typename T, int DP, int NW, bool kSplit>
 __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 || NW < 4 ? 2 : 3) k_attention(const AttnRun A) {
     constexpr int NT = 64 * NW, KT = tile_rows(DP, NW), KB = KT / 32, NBUF = tile_buffers(NW);
@@ -155,10 +155,16 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 && NW == 1 ? 1 : DP == 128 
                         }
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const half8<T> p = to_operand<T>(s[b], x);
+                            // P rounded once costs the output as much precision as its own rounding does, and the output's error
+                            // comes back in every gradient: what the first product left follows in a second
+                            const half8<T> p = to_operand<T>(s[b], x), rest = rest_operand<T>(s[b], x, p);
+                            half8<T> f[DP / 32];
 #pragma unroll
-                            for (int d = 0; d < DP / 32; ++d)
-                                o[d] = mfma(column_fragment<T, DP>(vt, 32 * b + 16 * x, 32 * d, lane), p, o[d]);
+                            for (int d = 0; d < DP / 32; ++d) f[d] = column_fragment<T, DP>(vt, 32 * b + 16 * x, 32 * d, lane);
+#pragma unroll
+                            for (int d = 0; d < DP / 32; ++d) o[d] = mfma(f[d], p, o[d]);
+#pragma unroll
+                            for (int d = 0; d < DP / 32; ++d) o[d] = mfma(f[d], rest, o[d]);
                         }
                     }
                 }
